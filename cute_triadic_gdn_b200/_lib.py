@@ -1,5 +1,5 @@
 """Loads the compiled parts of the package: libtgdn_b200.so through ctypes (`lib`: the C ABI declared in include/tgdn.h) and the
-host path _tgdn_torch.so, a torch extension (`host`: operators, autograd and launches; csrc/tgdn_torch.cpp).
+host path _tgdn_torch.so, a torch extension (`host`: operators, autograd and launches; csrc/tgdn_torch*.cpp).
 
 The library is the only implementation of the hot path: there is no fallback.  If the shared object is missing it is
 built once with nvcc (cute_triadic_gdn_b200/build.py); if that is impossible the import fails loudly.
@@ -39,11 +39,31 @@ SIGNATURES = {
     "tgdn_bwd_recurrent_state": (_I, [_P] * 10 + [_F, _P, _P] + [_I] * 6 + [_P] * 8),
     "tgdn_bwd_state_grads": (_I, [_P] * 10 + [_F, _P] + [_I] * 5 + [_P] * 5),
     "tgdn_bwd_matrix": (_I, [_P] * 16 + [_F, _P] + [_I] * 5 + [_P] * 7),
+    "tgdn_scan_carry_floats": (_L, [_I, _I, _I]),
+    "tgdn_scan_map": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "tgdn_scan_fwd": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "tgdn_scan_bwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I] + [_P] * 7),
+    "tgdn_scan_step": (_I, [_P, _P, _I, _I, _P, _P, _P]),
+    "tgdn_norm_scratch_floats": (_L, [_L, _I]),
+    "tgdn_residual_norm_fwd": (_I, [_P, _P, _P, _P, _F, _L, _I, _F, _P, _P, _P, _P]),
+    "tgdn_residual_norm_bwd": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _F, _P, _L, _I, _P, _P, _P, _P, _P, _L, _P]),
+    "tgdn_gated_norm_fwd": (_I, [_P, _P, _I, _P, _P, _P, _F, _L, _I, _F, _P, _I, _P, _P]),
+    "tgdn_gated_norm_bwd": (_I, [_P, _P, _I, _P, _P, _P, _F, _P, _L, _I, _P, _P, _P, _P, _P, _L, _P]),
     "tgdn_selftest_mma": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "tgdn_selftest_tma": (_I, [_P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P]),
     "tgdn_selftest_wait": (_I, [_c.c_longlong, _P, _P]),
     "tgdn_selftest_role": (_I, [_c.c_longlong, _P, _P]),
 }
+
+
+class Rows(_c.Structure):
+    """tgdn_rows of include/tgdn.h."""
+    _fields_ = [("data", _P), ("inner", _L), ("stride_outer", _L), ("stride_inner", _L), ("type", _I)]
+
+
+class Vector(_c.Structure):
+    """tgdn_vector of include/tgdn.h."""
+    _fields_ = [("data", _P), ("type", _I)]
 
 
 class TgdnError(RuntimeError):

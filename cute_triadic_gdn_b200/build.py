@@ -1,5 +1,5 @@
 """Builds, in-tree, libtgdn_b200.so (sm_100a only) from csrc/*.cu with nvcc and the package's host path _tgdn_torch.so from
-csrc/tgdn_torch.cpp with the host compiler (against the torch that is installed; linked with the first).
+csrc/*.cpp with the host compiler (against the torch that is installed; linked with the first).
 
     python -m cute_triadic_gdn_b200.build [--force] [--verbose]
 
@@ -41,6 +41,10 @@ def _nvcc():
 
 def _sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith(".cu"))
+
+
+def _host_sources():
+    return sorted(f for f in os.listdir(CSRC) if f.endswith(".cpp"))
 
 
 def _torch_root():
@@ -97,23 +101,23 @@ def _build_locked(verbose):
             print(r.stderr)
         return obj
 
-    def compile_host():
-        torch_root, obj = _torch_root(), os.path.join(BUILD, "tgdn_torch.o")
+    def compile_host(src):
+        torch_root, obj = _torch_root(), os.path.join(BUILD, src[:-4] + ".host.o")
         cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc)))
         inc = [os.path.join(torch_root, "include"), os.path.join(torch_root, "include", "torch", "csrc", "api", "include"),
                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
         cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unknown-pragmas",
                f"-DTORCH_EXTENSION_NAME={HOST_MODULE}", "-DTORCH_API_INCLUDE_EXTENSION_H", *[f for i in inc for f in ("-isystem", i)],
-               "-c", os.path.join(CSRC, "tgdn_torch.cpp"), "-o", obj]
+               "-c", os.path.join(CSRC, src), "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"the host compiler failed on tgdn_torch.cpp:\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"the host compiler failed on {src}:\n{r.stdout}\n{r.stderr}")
         return obj
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
-        host_obj = pool.submit(compile_host)
+        host_objs = [pool.submit(compile_host, src) for src in _host_sources()]
         objs = list(pool.map(compile_one, _sources()))
-        host_obj = host_obj.result()
+        host_objs = [obj.result() for obj in host_objs]
     tmp = OUT + f".tmp{os.getpid()}"
     cmd = [nvcc, "-shared", "-o", tmp, *objs, "-lcudart"]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -122,7 +126,7 @@ def _build_locked(verbose):
     os.replace(tmp, OUT)                               # atomic: a concurrent dlopen sees the old or the new file, never half of one
     tmp = HOST_OUT + f".tmp{os.getpid()}"
     lib = os.path.join(_torch_root(), "lib")
-    cmd = [shutil.which("g++") or "c++", "-shared", "-o", tmp, host_obj, "-L" + PKG, "-l:libtgdn_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + lib,
+    cmd = [shutil.which("g++") or "c++", "-shared", "-o", tmp, *host_objs, "-L" + PKG, "-l:libtgdn_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + lib,
            "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -181,6 +181,7 @@ extern "C" const char* tgdn_error_string(int code) {
     case TGDN_ERR_SCRATCH: return "scratch buffer missing or too small";
     case TGDN_ERR_DEVICE: return "the current device is not compute capability 10.x (sm_100a kernels)";
     case TGDN_ERR_STATIC_LIMIT: return "the problem needs more scratch than the library's built-in static buffer holds";
+    case TGDN_ERR_TYPE: return "unsupported element type or pair of types";
     default: break;
   }
   if (code <= -1000) {
@@ -191,7 +192,7 @@ extern "C" const char* tgdn_error_string(int code) {
   return buf;
 }
 
-extern "C" int tgdn_abi_version(void) { return 101; }
+extern "C" int tgdn_abi_version(void) { return 102; }
 extern "C" int tgdn_gate_item_floats(int E) { return tgdn::gate_item_floats(E); }
 
 extern "C" int tgdn_device_status(int* host_status) {

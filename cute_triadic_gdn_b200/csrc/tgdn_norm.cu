@@ -1,0 +1,191 @@
+// The norm before a block (tgdn_norm.cuh): residual stream, norm and weight in one pass, and the sums over rows that both norms leave.
+#include "tgdn_norm.cuh"
+
+namespace tgdn {
+
+template <typename TX, typename TR, int VEC, int K, int MAXT>
+__global__ void __launch_bounds__(MAXT) residual_fwd_kernel(NormParams p) {
+  __shared__ float red[2][NORM_MAX_WARPS];
+  const int tpr = p.tpr, lane = threadIdx.x % tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
+  float w[K][VEC], c[K][VEC];
+  load_small<VEC, K>(p.weight, 1.f, lane, tpr, p.N, w);
+  load_small<VEC, K>(p.scale, p.scale_value, lane, tpr, p.N, c);
+  int phase = 0;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < p.rows; base += static_cast<int64_t>(gridDim.x) * groups) {
+    const int64_t row = base + group;
+    const bool ok = row < p.rows;
+    float x[K][VEC], r[K][VEC];
+    const uint32_t rr = ok ? static_cast<uint32_t>(row) : 0u;
+    load_row<TX, VEC, K>(static_cast<const TX*>(p.x.p) + p.x.at(rr), ok, lane, tpr, p.N, x);
+    load_row<TR, VEC, K>(static_cast<const TR*>(p.other.p) + p.other.at(rr), ok, lane, tpr, p.N, r);
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        r[k][i] = fmaf(c[k][i], x[k][i], r[k][i]);
+        ss = fmaf(r[k][i], r[k][i], ss);
+      }
+    store_row<TR, VEC, K>(static_cast<TR*>(p.stream) + row * p.N, ok, lane, tpr, p.N, r);
+    const float inv = rsqrtf(fmaf(row_sum(ss, tpr, red, phase), p.inv_n, p.eps));
+    phase ^= 1;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) r[k][i] *= inv * w[k][i];
+    store_row<TX, VEC, K>(static_cast<TX*>(p.out) + row * p.N, ok, lane, tpr, p.N, r);
+    if (ok && lane == 0 && p.rstd) p.rstd[row] = inv;
+  }
+}
+
+template <typename TX, typename TR, int VEC, int K, int MAXT>
+__global__ void __launch_bounds__(MAXT) residual_bwd_kernel(NormParams p) {
+  __shared__ float red[2][NORM_MAX_WARPS];
+  __shared__ float area[NORM_BLOCK * VEC * K];
+  const int tpr = p.tpr, lane = threadIdx.x % tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
+  float w[K][VEC], c[K][VEC], dw[K][VEC], dc[K][VEC];
+  load_small<VEC, K>(p.weight, 1.f, lane, tpr, p.N, w);
+  load_small<VEC, K>(p.scale, p.scale_value, lane, tpr, p.N, c);
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dw[k][i] = dc[k][i] = 0.f;
+  int phase = 0;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < p.rows; base += static_cast<int64_t>(gridDim.x) * groups) {
+    const int64_t row = base + group;
+    const bool ok = row < p.rows;
+    const uint32_t rr = ok ? static_cast<uint32_t>(row) : 0u;
+    float n[K][VEC], dy[K][VEC], ds[K][VEC], x[K][VEC];
+    load_row<TR, VEC, K>(static_cast<const TR*>(p.stream) + rr * static_cast<int64_t>(p.N), ok, lane, tpr, p.N, n);
+    load_row<TX, VEC, K>(static_cast<const TX*>(p.dy.p) + p.dy.at(rr), ok && p.dy.p, lane, tpr, p.N, dy);
+    load_row<TR, VEC, K>(static_cast<const TR*>(p.dstream.p) + p.dstream.at(rr), ok && p.dstream.p, lane, tpr, p.N, ds);
+    if (p.sums1) load_row<TX, VEC, K>(static_cast<const TX*>(p.x.p) + p.x.at(rr), ok, lane, tpr, p.N, x);
+    const float inv = ok ? p.rstd[row] : 0.f;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        n[k][i] *= inv;
+        dw[k][i] = fmaf(dy[k][i], n[k][i], dw[k][i]);
+        dy[k][i] *= w[k][i];
+        s = fmaf(dy[k][i], n[k][i], s);
+      }
+    s = row_sum(s, tpr, red, phase) * p.inv_n;
+    phase ^= 1;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        ds[k][i] = fmaf(inv, fmaf(-n[k][i], s, dy[k][i]), ds[k][i]);
+        if (p.sums1) dc[k][i] = fmaf(ds[k][i], x[k][i], dc[k][i]);
+        dy[k][i] = ds[k][i] * c[k][i];
+      }
+    store_row<TR, VEC, K>(static_cast<TR*>(p.dother) + row * p.N, ok, lane, tpr, p.N, ds);
+    if (p.dx) store_row<TX, VEC, K>(static_cast<TX*>(p.dx) + row * p.N, ok, lane, tpr, p.N, dy);
+  }
+  if (p.sums0) leave_sums<VEC, K>(dw, p.sums0, area, lane, group, groups, tpr, p.N);
+  if (p.sums1) leave_sums<VEC, K>(dc, p.sums1, area, lane, group, groups, tpr, p.N);
+}
+
+// Column sums of the partials, in the order of the blocks: thread (i, j) adds up every 32nd partial of channel j from the i-th on, then
+// the 32 of a channel are added up in order.  out0 = factor0 sum, out1 = factor1 sum (one or both).
+constexpr int SUM_ROWS = 32;
+struct SumParams {
+  const float* partials;
+  int blocks, N;
+  SmallVector factor0, factor1;
+  float value0, value1;
+  void *out0, *out1;
+  int type0, type1;
+};
+__global__ void __launch_bounds__(32 * SUM_ROWS) norm_sums_kernel(SumParams p) {
+  __shared__ float part[SUM_ROWS][33];
+  const int j = threadIdx.x & 31, i = threadIdx.x >> 5, c = blockIdx.x * 32 + j;
+  float s = 0.f;
+  if (c < p.N)
+    for (int b = i; b < p.blocks; b += SUM_ROWS) s += p.partials[static_cast<int64_t>(b) * p.N + c];
+  part[i][j] = s;
+  __syncthreads();
+  if (i == 0 && c < p.N) {
+    s = 0.f;
+    for (int k = 0; k < SUM_ROWS; ++k) s += part[k][j];
+    if (p.out0) store_any(p.out0, p.type0, c, s * p.factor0.get(c, p.value0));
+    if (p.out1) store_any(p.out1, p.type1, c, s * p.factor1.get(c, p.value1));
+  }
+}
+
+int norm_add_up(const float* partials, int blocks, int N, const tgdn_vector* f0, float v0, void* out0, int t0, const tgdn_vector* f1, float v1, void* out1,
+           int t1, cudaStream_t st) {
+  SumParams q{partials, blocks, N, small(f0), small(f1), v0, v1, out0, out1, t0, t1};
+  norm_sums_kernel<<<(N + 31) / 32, 32 * SUM_ROWS, 0, st>>>(q);
+  return tgdn_cuda_error(cudaGetLastError());
+}
+
+}  // namespace tgdn
+
+using namespace tgdn;
+
+namespace {
+TGDN_LAUNCHER(ResidualFwd, residual_fwd_kernel);
+TGDN_LAUNCHER(ResidualBwd, residual_bwd_kernel);
+}  // namespace
+
+extern "C" int64_t tgdn_norm_scratch_floats(int64_t rows, int N) {
+  if (check_norm(rows, N)) return 0;
+  int most = 0;
+  for (const int vec : {4, 8}) {                  // whichever layout the alignment allows
+    for (const bool vectors : {true, false}) {
+      const int b = norm_blocks(norm_shape(N, vectors, vec), rows);
+      if (b > most) most = b;
+    }
+  }
+  return 2 * static_cast<int64_t>(most) * N;
+}
+
+extern "C" int tgdn_residual_norm_fwd(const tgdn_rows* host_x, const tgdn_rows* host_residual, const tgdn_vector* host_weight,
+                                      const tgdn_vector* host_scale, float scale_value, int64_t rows, int N, float eps, void* y,
+                                      void* stream_out, float* rstd, void* stream) {
+  TGDN_TRY(check_rows(host_x, true)); TGDN_TRY(check_rows(host_residual, true));
+  TGDN_TRY(check_vector(host_weight)); TGDN_TRY(check_vector(host_scale)); TGDN_TRY(check_norm(rows, N));
+  if (!y || !stream_out) return TGDN_ERR_NULL;
+  if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
+  const int xt = host_x->type, rt = host_residual->type;
+  const tgdn_rows yo = dense(y, xt, rows, N), so = dense(stream_out, rt, rows, N);
+  const NormShape s = norm_shape(N, vectors_ok(N, vec_of(xt), {host_x, host_residual, &yo, &so}), vec_of(xt));
+  NormParams p = norm_params(rows, N, eps, s, host_weight, host_scale, scale_value);
+  p.x = rows_at(host_x); p.other = rows_at(host_residual); p.out = y; p.stream = stream_out; p.rstd = rstd;
+  return launch_types<ResidualFwd>(xt, rt, s, norm_blocks(s, rows), p, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tgdn_residual_norm_bwd(const void* stream_in, int stream_type, const tgdn_rows* host_x, int x_type, const tgdn_rows* host_dy,
+                                      const tgdn_rows* host_dstream, const tgdn_vector* host_weight, const tgdn_vector* host_scale,
+                                      float scale_value, const float* rstd, int64_t rows, int N, void* dresidual, void* dx,
+                                      const tgdn_vector* host_dweight, const tgdn_vector* host_dscale, float* scratch, int64_t scratch_floats,
+                                      void* stream) {
+  TGDN_TRY(check_rows(host_dy, false)); TGDN_TRY(check_rows(host_dstream, false));
+  TGDN_TRY(check_vector(host_weight)); TGDN_TRY(check_vector(host_scale)); TGDN_TRY(check_vector(host_dweight)); TGDN_TRY(check_vector(host_dscale));
+  TGDN_TRY(check_norm(rows, N));
+  const bool want_w = host_dweight && host_dweight->data, want_c = host_dscale && host_dscale->data;
+  TGDN_TRY(check_rows(host_x, want_c));
+  if (!stream_in || !rstd || !dresidual) return TGDN_ERR_NULL;
+  if (!type_known(stream_type) || !type_known(x_type)) return TGDN_ERR_TYPE;
+  if (want_c && host_x->type != x_type) return TGDN_ERR_TYPE;
+  if ((host_dy && host_dy->data && host_dy->type != x_type) || (host_dstream && host_dstream->data && host_dstream->type != stream_type)) return TGDN_ERR_TYPE;
+  if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
+  const tgdn_rows si = dense(stream_in, stream_type, rows, N), dr = dense(dresidual, stream_type, rows, N), dxo = dense(dx, x_type, rows, N);
+  const NormShape s = norm_shape(N, vectors_ok(N, vec_of(x_type), {&si, &dr, &dxo, host_dy, host_dstream, want_c ? host_x : nullptr}), vec_of(x_type));
+  const int blocks = norm_blocks(s, rows);
+  if ((want_w || want_c) && (!scratch || scratch_floats < 2 * static_cast<int64_t>(blocks) * N)) return TGDN_ERR_SCRATCH;
+  NormParams p = norm_params(rows, N, 0.f, s, host_weight, host_scale, scale_value);
+  p.x = rows_at(want_c ? host_x : nullptr); p.dy = rows_at(host_dy); p.dstream = rows_at(host_dstream);
+  p.stream = const_cast<void*>(stream_in); p.rstd = const_cast<float*>(rstd); p.dother = dresidual; p.dx = dx;
+  p.sums0 = want_w ? scratch : nullptr;
+  p.sums1 = want_c ? scratch + static_cast<int64_t>(blocks) * N : nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TGDN_TRY(launch_types<ResidualBwd>(x_type, stream_type, s, blocks, p, st));
+  if (want_w) TGDN_TRY(norm_add_up(p.sums0, blocks, N, nullptr, 1.f, const_cast<void*>(host_dweight->data), host_dweight->type, nullptr, 1.f, nullptr, 0, st));
+  if (want_c) TGDN_TRY(norm_add_up(p.sums1, blocks, N, nullptr, 1.f, const_cast<void*>(host_dscale->data), host_dscale->type, nullptr, 1.f, nullptr, 0, st));
+  return 0;
+}
+

@@ -14,80 +14,13 @@
 //
 // The device work is libtgdn_b200, with which this file is linked: the entry points of include/tgdn.h in the forms of tgdn_host.h (token
 // ranges of longer rows, rows of any alignment, the glue's backward in one pass).
-#include <torch/extension.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/library.h>
-
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-
-#include <cmath>
-#include <cstdlib>
-#include <cstring>
-#include <optional>
-#include <stdexcept>
-#include <string>
-#include <tuple>
-#include <vector>
-
-#include "tgdn_host.h"
+#include "tgdn_torch.h"
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace tgdn_torch;
 
 constexpr int64_t CHUNK = 64, HEAD_DIM = 128;
-
-// ---- errors -----------------------------------------------------------------------------------------------------------
-// The package raises AssertionError from the argument checks of the core (as the reference does), ValueError for
-// packed-row and device / E problems, and TgdnError (_lib.py) when the library rejects a call.
-struct AssertFail : std::runtime_error { using std::runtime_error::runtime_error; };
-struct LibraryFail : std::runtime_error { using std::runtime_error::runtime_error; };
-
-py::handle library_error;                                  // TgdnError, set by _lib.py
-void set_python_error(const AssertFail& e) { PyErr_SetString(PyExc_AssertionError, e.what()); }
-void set_python_error(const LibraryFail& e) { PyErr_SetString(library_error ? library_error.ptr() : PyExc_RuntimeError, e.what()); }
-
-// Impl::forward and Impl::backward as an autograd function.  A backward runs under torch's engine, which keeps the class of a Python
-// error only: the two above are turned into one there (elsewhere the module's translator does it).
-template <typename Impl>
-struct Differentiable : public torch::autograd::Function<Differentiable<Impl>> {
-  template <typename... Args>
-  static auto forward(AutogradContext* ctx, Args&&... args) { return Impl::forward(ctx, std::forward<Args>(args)...); }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    try {
-      return Impl::backward(ctx, std::move(grads));
-    } catch (const AssertFail& e) {
-      rethrow(e);
-    } catch (const LibraryFail& e) {
-      rethrow(e);
-    }
-  }
-  template <typename Fail>
-  [[noreturn]] static void rethrow(const Fail& e) {
-    py::gil_scoped_acquire gil;
-    set_python_error(e);
-    python_error error;
-    error.persist();
-    throw error;
-  }
-};
-
-void check_rc(int rc, const char* what) {
-  if (rc != 0) throw LibraryFail(std::string(what) + ": " + tgdn_error_string(rc) + " (code " + std::to_string(rc) + ")");
-}
-
-std::string shape_of(const Tensor& t) {
-  std::string s = "(";
-  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
-  return s + ")";
-}
-
-#define TGDN_ASSERT(cond, ...) do { if (!(cond)) throw AssertFail(c10::str(__VA_ARGS__)); } while (0)
 
 // Shapes, dtypes, contiguity and device of the seven inputs; names the first thing that is off (same conditions as
 // ops/gdn_joint.py:235-249 of the reference).
@@ -139,15 +72,6 @@ bool save_masks() {
 }
 
 // ---- the stages -------------------------------------------------------------------------------------------------------
-template <typename T = void>
-T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
-template <typename T = void>
-T* ptr(const OptTensor& t) { return t.has_value() ? ptr<T>(*t) : nullptr; }
-const float* fptr(const Tensor& t) { return ptr<float>(t); }
-bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-
 struct Dims {
   int B, T, H, E, NC, row_tokens, n_docs;
   int64_t blocks() const { return 128 / tgdn_value_block(E); }      // value blocks of the reverse recurrence
@@ -163,8 +87,6 @@ Dims dims(const Tensor& q, const Tensor& k2, const OptTensor& token_map, const O
   d.n_docs = has(chunk_starts) ? static_cast<int>(chunk_starts->numel() - 1) : 0;
   return d;
 }
-
-Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dtype) { return at::empty(sizes, like.options().dtype(dtype)); }
 
 struct Masks { Tensor gc, AP, Pm; };
 
@@ -403,16 +325,6 @@ std::vector<Tensor> call_joint_bwd(at::TensorList saved, const Tensor& dO, doubl
 std::vector<Tensor> joint_bwd_entry(at::TensorList saved, const Tensor& dO, double scale, const OptTensor& chunk_starts,
                                     const OptTensor& token_map, bool covered) {
   return joint_bwd(saved.vec(), dO, scale, chunk_starts, token_map, covered);
-}
-
-Tensor or_undefined(const OptTensor& t) { return has(t) ? *t : Tensor(); }
-OptTensor or_nullopt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-
-bool any_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : ts)
-    if (t->requires_grad()) return true;
-  return false;
 }
 
 // Differentiates joint_fwd (reference: ops/joint_torch_ops.py:50-80, ops/gdn_joint.py:201-232).
@@ -909,6 +821,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("conv_call", &call_conv_fwd, nogil);
   m.def("conv_norm_call", &call_norm_fwd, nogil);
   m.def("prepare_documents", &prepare_documents, nogil);
+  bind_block_operators(m);
   // the stages one by one, with every optional argument given
   m.def("run_masks", [](const Tensor& q, const Tensor& k, const Tensor& k2, const Tensor& q2, const Tensor& g, const Tensor& beta,
                         double scale, const OptTensor& token_map) {

@@ -30,6 +30,7 @@ extern "C" {
 #define TGDN_ERR_SCRATCH (-5)     /* scratch buffer missing or too small */
 #define TGDN_ERR_DEVICE (-6)      /* the current device is not compute capability 10.x */
 #define TGDN_ERR_STATIC_LIMIT (-7) /* the problem needs more scratch than the library's built-in static buffer holds */
+#define TGDN_ERR_TYPE (-8)        /* an element type, or a pair of them, that the kernels do not come in */
 
 /* Human-readable text for a return code of this library. */
 const char* tgdn_error_string(int code);
@@ -197,6 +198,83 @@ int tgdn_bwd_matrix(const void* q, const void* k, const void* dO, const void* dU
                     const void* dkq, const float* da, const float* dc, const float* dd, const float* dr, float scale,
                     const int32_t* chunk_map, int B, int T, int H, int E, int NC, void* dq, void* dk, float* dk2,
                     float* dq2, float* dg, float* dbeta, void* stream);
+
+/* ---- operators around the core -------------------------------------------------------------------------------------
+ * No counterparts in the reference, which leaves the block around the core to its caller.  Element types and strides are the caller's:
+ * tensors of rows come as tgdn_rows, small vectors over the channels as tgdn_vector (both host structures, read during the call).
+ * Pairs of types: f32 with f32; bf16 or f16 with itself or with f32 (named per entry). */
+#define TGDN_F32 0
+#define TGDN_BF16 1
+#define TGDN_F16 2
+
+/* Rows of consecutive channels.  Row r starts (r / inner) * stride_outer + (r % inner) * stride_inner elements behind `data`; the scan
+ * calls take a (B, T, D) tensor, stride_outer from batch row to batch row and stride_inner from token to token (inner is not read).
+ * Strides may be zero; any alignment of whole elements will do (rows on 16-byte boundaries, or of pairs in the scan, are faster).
+ * data = NULL: no tensor. */
+typedef struct {
+  const void* data;
+  int64_t inner, stride_outer, stride_inner;
+  int type;
+} tgdn_rows;
+
+typedef struct {
+  const void* data; /* consecutive elements; written where the argument is an output; NULL: none */
+  int type;
+} tgdn_vector;
+
+/* Gated linear recurrence per channel: h[t] = exp(g[t]) h[t-1] + x[t] over (B, T, D), states f32.  (x, g): types f32 with f32, bf16 or
+ * f16 with themselves or f32.  Dense rows: map = NULL, sequences = B.  Packed rows: B = 1, map (T) int32 from tgdn_scan_map, sequences =
+ * n_docs; every document starts from its own state.  initial: f32 (sequences, D) or NULL (zero); final_state: f32 (sequences, D) or NULL;
+ * carry: tgdn_scan_carry_floats(B, T, D) floats that the backward reads (the state before every TGDN_SCAN_TILE tokens), or NULL.
+ * h: (B, T, D) contiguous, x's type. */
+#define TGDN_SCAN_TILE 128
+int64_t tgdn_scan_carry_floats(int B, int T, int D);
+int tgdn_scan_map(const void* cu_seqlens, int cu_is_int64, int n_docs, int T, int32_t* map, uint8_t* valid, void* stream);
+int tgdn_scan_fwd(const tgdn_rows* host_x, const tgdn_rows* host_g, const int32_t* map, int n_docs, int B, int T, int D,
+                  const float* initial, void* h, float* final_state, float* carry, void* stream);
+
+/* The gradients: dh (x's type) and dfinal (f32 (sequences, D), or NULL: zero) -> dx, dg (contiguous, the types of x and g) and, where
+ * dinitial is not NULL, dinitial (f32 (sequences, D)). */
+int tgdn_scan_bwd(const tgdn_rows* host_x, const tgdn_rows* host_g, const tgdn_rows* host_dh, const int32_t* map, int n_docs, int B,
+                  int T, int D, const float* initial, const float* carry, const float* dfinal, void* dx, void* dg, float* dinitial,
+                  void* stream);
+
+/* One token of B sequences on a resident state: state (B, D) f32 <- exp(g) state + x in place, h (B, D) = the new state in x's type.
+ * x, g: (B, 1, D). */
+int tgdn_scan_step(const tgdn_rows* host_x, const tgdn_rows* host_g, int B, int D, float* state, void* h, void* stream);
+
+/* Norms before and after a block over `rows` rows of N <= TGDN_NORM_MAX_CHANNELS channels.  weight NULL: ones.  The scale is a vector
+ * over the channels or, where that is NULL, the number scale_value.  rstd (f32, one a row) goes from the forward to the backward (NULL:
+ * no backward follows).  Sums over rows: scratch of tgdn_norm_scratch_floats(rows, N) floats, added up in a fixed order; it may be NULL
+ * where neither dweight nor dscale is asked for. */
+#define TGDN_NORM_MAX_CHANNELS 16384
+int64_t tgdn_norm_scratch_floats(int64_t rows, int N);
+
+/* Before a block: stream_out = residual + scale x (residual's type: x's or f32), y = stream / sqrt(mean(stream^2) + eps) weight (x's type),
+ * the norm taken before the stream is rounded.  Outputs contiguous. */
+int tgdn_residual_norm_fwd(const tgdn_rows* host_x, const tgdn_rows* host_residual, const tgdn_vector* host_weight,
+                           const tgdn_vector* host_scale, float scale_value, int64_t rows, int N, float eps, void* y,
+                           void* stream_out, float* rstd, void* stream);
+/* Its gradients from dy and dstream (either may be NULL: zero): dresidual (the stream's type), dx = scale dresidual (NULL: not wanted),
+ * dweight and dscale (NULL: not wanted; x is read for dscale only). */
+int tgdn_residual_norm_bwd(const void* stream_in, int stream_type, const tgdn_rows* host_x, int x_type, const tgdn_rows* host_dy,
+                           const tgdn_rows* host_dstream, const tgdn_vector* host_weight, const tgdn_vector* host_scale,
+                           float scale_value, const float* rstd, int64_t rows, int N, void* dresidual, void* dx,
+                           const tgdn_vector* host_dweight, const tgdn_vector* host_dscale, float* scratch, int64_t scratch_floats,
+                           void* stream);
+
+/* After a block: out = [residual +] scale (x / sqrt(mean(x^2) + eps) weight act(gate)); out_type: x's or f32, and the residual's. */
+#define TGDN_ACT_NONE 0
+#define TGDN_ACT_SILU 1
+#define TGDN_ACT_SIGMOID 2
+int tgdn_gated_norm_fwd(const tgdn_rows* host_x, const tgdn_rows* host_gate, int activation, const tgdn_vector* host_weight,
+                        const tgdn_rows* host_residual, const tgdn_vector* host_scale, float scale_value, int64_t rows, int N,
+                        float eps, void* out, int out_type, float* rstd, void* stream);
+/* Its gradients from dout (the type of out): dx, dgate (x's type), dweight and dscale (NULL: not wanted).  The residual's is dout. */
+int tgdn_gated_norm_bwd(const tgdn_rows* host_x, const tgdn_rows* host_gate, int activation, const tgdn_rows* host_dout,
+                        const tgdn_vector* host_weight, const tgdn_vector* host_scale, float scale_value, const float* rstd,
+                        int64_t rows, int N, void* dx, void* dgate, const tgdn_vector* host_dweight, const tgdn_vector* host_dscale,
+                        float* scratch, int64_t scratch_floats, void* stream);
 
 #ifdef __cplusplus
 }
