@@ -157,19 +157,9 @@ NormShape norm_shape(int N, bool vectors, int vec_elements) {
   return s;
 }
 
-int sm_count() {
-  static int cached[64] = {0};
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (dev >= 0 && dev < 64 && cached[dev]) return cached[dev];
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-  if (dev >= 0 && dev < 64) cached[dev] = n;
-  return n;
-}
-
 // Blocks of a pass: as many as hold the rows, at most two thousand threads' worth on every SM.
 int norm_blocks(const NormShape& s, int64_t rows) {
-  const int64_t want = (rows + s.groups - 1) / s.groups, most = static_cast<int64_t>(sm_count()) * (2048 / s.threads > 0 ? 2048 / s.threads : 1);
+  const int64_t want = (rows + s.groups - 1) / s.groups, most = static_cast<int64_t>(tgdn_sm_count()) * (2048 / s.threads > 0 ? 2048 / s.threads : 1);
   return static_cast<int>(want < most ? want : most);
 }
 

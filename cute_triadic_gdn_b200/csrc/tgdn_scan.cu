@@ -22,12 +22,14 @@ namespace tgdn {
 
 constexpr int SCAN_ROWS = 16;                    // rows a warp holds
 constexpr int SCAN_WARPS = 8;
+constexpr int SCAN_MAX_CLUSTER = 8;              // blocks along time that exchange their maps
 constexpr int SCAN_TILE = SCAN_ROWS * SCAN_WARPS;
 static_assert(SCAN_TILE == TGDN_SCAN_TILE, "rows between two saved states");
 
 struct ScanIn {
   const void* p;
-  int64_t sb, st;                                // elements from one batch row, and from one token, to the next
+  int64_t sb;                                    // elements from one batch row, and from one token, to the next
+  int st;
 };
 
 struct ScanParams {
@@ -41,32 +43,87 @@ struct ScanParams {
   void* dx;
   void* dg;
   float* dinitial;
-  int B, T, D, n_docs, slices, tiles;
+  int B, T, D, n_docs, slices, tiles, cluster;
 };
 
+// A lane's channels of one row.  Pairs go through the two-wide f32 instructions: the kernels would be bound by the issue of
+// instructions otherwise (one at a time: 37 an element forward, 102 us at 8 x 4096 x 2048 in bf16; see the note at the launch).
+template <int VEC>
+struct alignas(4 * VEC) Lanes {
+  float v[VEC];
+};
+__device__ __forceinline__ float2 pair_of(const Lanes<2>& l) { return make_float2(l.v[0], l.v[1]); }
+__device__ __forceinline__ Lanes<2> lanes_of(float2 p) { return {{p.x, p.y}}; }
+__device__ __forceinline__ Lanes<2> fma(const Lanes<2>& a, const Lanes<2>& b, const Lanes<2>& c) { return lanes_of(__ffma2_rn(pair_of(a), pair_of(b), pair_of(c))); }
+__device__ __forceinline__ Lanes<2> mul(const Lanes<2>& a, const Lanes<2>& b) { return lanes_of(__fmul2_rn(pair_of(a), pair_of(b))); }
+__device__ __forceinline__ Lanes<2> add(const Lanes<2>& a, const Lanes<2>& b) { return lanes_of(__fadd2_rn(pair_of(a), pair_of(b))); }
+__device__ __forceinline__ Lanes<1> fma(const Lanes<1>& a, const Lanes<1>& b, const Lanes<1>& c) { return {{fmaf(a.v[0], b.v[0], c.v[0])}}; }
+__device__ __forceinline__ Lanes<1> mul(const Lanes<1>& a, const Lanes<1>& b) { return {{__fmul_rn(a.v[0], b.v[0])}}; }
+__device__ __forceinline__ Lanes<1> add(const Lanes<1>& a, const Lanes<1>& b) { return {{__fadd_rn(a.v[0], b.v[0])}}; }
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> all(float f) {
+  Lanes<VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r.v[i] = f;
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> load_f32(const float* p, bool ok) {
+  Lanes<VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r.v[i] = ok ? p[i] : 0.f;
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ void store_f32(float* p, const Lanes<VEC>& l) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) p[i] = l.v[i];
+}
+
+__device__ __forceinline__ float power_of_two(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
 // exp(g).  Near zero as 1 + (g + g^2/2 + ...): the sum is rounded once, to nearest, while the hardware's power of two errs by up to two
 // units to one side, and such errors add up over as many tokens as the state remembers (a thousand tokens at g = -1e-3: 2e-5 where
 // roundings to nearest leave 1e-6).  Beyond 1/8 a state remembers eight tokens at most and the power of two is good enough.  The series
-// to the fifth power is 2^-28 off at 1/8.
-__device__ __forceinline__ float decay(float g) {
-  float s = fmaf(g, 1.f / 120.f, 1.f / 24.f);
-  s = fmaf(g, s, 1.f / 6.f);
-  s = fmaf(g, s, 0.5f);
-  s = fmaf(g, s, 1.f);
-  s = fmaf(g, s, 1.f);
-  return fabsf(g) < 0.125f ? s : exp2f(g * 1.4426950408889634f);
-}
-
+// to the fifth power is 2^-28 off at 1/8.  (Decays below 2^-126 are zero.)
 template <int VEC>
-struct Channels {
-  float v[VEC];
-};
+__device__ __forceinline__ Lanes<VEC> decay(const Lanes<VEC>& g) {
+  Lanes<VEC> s = fma(g, all<VEC>(1.f / 120.f), all<VEC>(1.f / 24.f));
+  s = fma(g, s, all<VEC>(1.f / 6.f));
+  s = fma(g, s, all<VEC>(0.5f));
+  s = fma(g, s, all<VEC>(1.f));
+  s = fma(g, s, all<VEC>(1.f));
+  const Lanes<VEC> t = mul(g, all<VEC>(1.4426950408889634f));
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) s.v[i] = fabsf(g.v[i]) < 0.125f ? s.v[i] : power_of_two(t.v[i]);
+  return s;
+}
+// The same for the rows of a tile; single channels two rows at a time.
+template <int VEC>
+__device__ __forceinline__ void decays(Lanes<VEC> (&g)[SCAN_ROWS]) {
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int r = 0; r < SCAN_ROWS; r += 2) {
+      const Lanes<2> a = decay<2>(Lanes<2>{{g[r].v[0], g[r + 1].v[0]}});
+      g[r].v[0] = a.v[0], g[r + 1].v[0] = a.v[1];
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < SCAN_ROWS; ++r) g[r] = decay<VEC>(g[r]);
+  }
+}
 
 // What a warp knows about the documents of its rows: bit r of `starts`, row r opens a document (whose number + 1 lane r holds); bit r of
 // `ends`, it closes one.
 struct RowDocs {
   uint32_t starts, ends;
   int code;
+  __device__ bool any() const { return (starts | ends) != 0; }
+  __device__ bool starts_at(int r) const { return starts >> r & 1; }
+  __device__ bool ends_at(int r) const { return ends >> r & 1; }
   __device__ int opened(int r) const { return __shfl_sync(0xffffffffu, code, r) - 1; }
   // The document before the one that opens at the next row; -1 where offsets that do not start at 0 leave none.
   __device__ int closed(int r) const { return __shfl_sync(0xffffffffu, code, r + 1) - 2; }
@@ -86,268 +143,375 @@ __device__ __forceinline__ RowDocs row_docs(const ScanParams& p, int t0, int lan
   return d;
 }
 
+// A tile's rows as they lie in memory: what a warp has in flight while it works on the tile before.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_rows(const ScanIn& in, int64_t base, int t0, int T_, bool active, float (&out)[SCAN_ROWS][VEC]) {
-  Pack<T, VEC> raw[SCAN_ROWS];
-  const T* p = static_cast<const T*>(in.p) + base;
-#pragma unroll
-  for (int r = 0; r < SCAN_ROWS; ++r)
-    raw[r] = active && t0 + r < T_ ? load_pack<T, VEC>(p + (t0 + r) * in.st) : zero_pack<T, VEC>();
-#pragma unroll
-  for (int r = 0; r < SCAN_ROWS; ++r)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[r][i] = to_f32(raw[r].v[i]);
-}
-
-// The maps of a block's warps, double-buffered: a tile's are written while slower warps still read the last one's.
-template <int VEC, int MAPS>
-struct alignas(16) WarpMaps {
-  float v[2][MAPS][SCAN_WARPS][32 * VEC];
-  int cut[2][2][SCAN_WARPS];                     // [buffer][forward, reverse][warp]: no state passes through
+struct RawRows {
+  typename RawOf<VEC * sizeof(T)>::type v[SCAN_ROWS];
 };
 
-template <int VEC>
-__device__ __forceinline__ Channels<VEC> read_map(const float* row, int lane) {
-  Channels<VEC> c;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) c.v[i] = row[lane * VEC + i];
-  return c;
+// Reads that nothing else in the kernel writes, in the order they stand in (volatile: they must be under way before the work that hides
+// them), and past L1: no line is read twice by a block.
+__device__ __forceinline__ void read_once(uint16_t& d, const void* p) { asm volatile("ld.global.nc.L1::no_allocate.b16 %0, [%1];" : "=h"(d) : "l"(p)); }
+__device__ __forceinline__ void read_once(uint32_t& d, const void* p) { asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(d) : "l"(p)); }
+__device__ __forceinline__ void read_once(uint2& d, const void* p) {
+  asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(d.x), "=r"(d.y) : "l"(p));
 }
-template <int VEC>
-__device__ __forceinline__ void write_map(float* row, int lane, const float (&v)[VEC]) {
+
+// Row r of a tile, for a stride below 2^31 elements (the launch checks): one wide product an address.  `stride` is made opaque once a tile, or
+// the compiler would keep its sixteen multiples in registers across the loop.
+template <typename T>
+__device__ __forceinline__ T* row_of(T* p, int r, int stride) { return p + static_cast<int64_t>(r) * stride; }
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+
+// Rows past T read as zeros.  Lanes past D read channel 0 (`base` says so) and store nothing.
+template <typename T, int VEC>
+__device__ __forceinline__ void request_rows(const ScanIn& in, int64_t base, int t0, int T_, RawRows<T, VEC>& raw) {
+  const T* p = static_cast<const T*>(in.p) + base + static_cast<int64_t>(t0) * in.st;
+  const int rows = T_ - t0, stride = opaque(in.st);
+  if (rows >= SCAN_ROWS) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) row[lane * VEC + i] = v[i];
+    for (int r = 0; r < SCAN_ROWS; ++r) read_once(raw.v[r], row_of(p, r, stride));
+  } else {
+#pragma unroll
+    for (int r = 0; r < SCAN_ROWS; ++r) {
+      raw.v[r] = {};
+      if (r < rows) read_once(raw.v[r], row_of(p, r, stride));
+    }
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack_rows(const RawRows<T, VEC>& raw, Lanes<VEC> (&out)[SCAN_ROWS]) {
+#pragma unroll
+  for (int r = 0; r < SCAN_ROWS; ++r) {
+    union { typename RawOf<VEC * sizeof(T)>::type raw; Pack<T, VEC> pack; } u;
+    u.raw = raw.v[r];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[r].v[i] = to_f32(u.pack.v[i]);
+  }
+}
+
+// A map of a run of rows in a lane's channels: c -> A c + H, or c -> H where a document's border lies in the run (`cut`, one value for all
+// channels: a state that is infinite or NaN must not pass, so a factor of zero would not do).
+template <int VEC, bool PACKED>
+struct Map {
+  Lanes<VEC> A, H;
+  int cut;
+  __device__ static Map identity() { return Map{all<VEC>(1.f), all<VEC>(0.f), 0}; }
+  __device__ void then(const Map& n) {           // this map, then n
+    H = PACKED && n.cut ? n.H : fma(n.A, H, n.H);
+    A = mul(A, n.A);
+    if (PACKED) cut |= n.cut;
+  }
+  __device__ void apply(Lanes<VEC>& c) const { c = PACKED && cut ? H : fma(A, c, H); }
+};
+
+// Maps in shared memory, of the block's warps and of the cluster's blocks; double-buffered, so that those of a round are written while
+// slower readers are still at the last round's.
+template <int VEC, int PARTS, bool PACKED>
+struct alignas(16) SharedMaps {
+  Lanes<VEC> A[2][PARTS][32], H[2][PARTS][32];
+  int cut[2][PARTS];
+  __device__ void put(int buf, int part, int lane, const Map<VEC, PACKED>& m) {
+    A[buf][part][lane] = m.A;
+    H[buf][part][lane] = m.H;
+    if (PACKED && lane == 0) cut[buf][part] = m.cut;
+  }
+  __device__ Map<VEC, PACKED> get(int buf, int part, int lane) const { return {A[buf][part][lane], H[buf][part][lane], PACKED ? cut[buf][part] : 0}; }
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_block_of_cluster(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void put_remote(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+__device__ __forceinline__ void put_remote(uint32_t at, float v, float w) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v), "f"(w) : "memory");
+}
+__device__ __forceinline__ void put_remote(uint32_t at, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+// The hardware's barrier over the blocks of a cluster, which all take every one: what was written before it is seen behind it.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Leaves the block's map with every block of the cluster, warp k at the k-th.
+template <int VEC, bool PACKED>
+__device__ __forceinline__ void put_in_cluster(SharedMaps<VEC, SCAN_MAX_CLUSTER, PACKED>& at, int buf, int rank, int blocks, int warp, int lane,
+                                               const Map<VEC, PACKED>& m) {
+  for (int k = warp; k < blocks; k += SCAN_WARPS) {
+    const uint32_t a = in_block_of_cluster(&at.A[buf][rank][lane], k), h = in_block_of_cluster(&at.H[buf][rank][lane], k);
+    if constexpr (VEC == 2) {
+      put_remote(a, m.A.v[0], m.A.v[1]);
+      put_remote(h, m.H.v[0], m.H.v[1]);
+    } else {
+      put_remote(a, m.A.v[0]);
+      put_remote(h, m.H.v[0]);
+    }
+    if (PACKED && lane == 0) put_remote(in_block_of_cluster(&at.cut[buf][rank], k), m.cut);
+  }
+}
+
+// Where a block stands: its slice of channels, its batch row, its place in the cluster.
+template <int VEC>
+struct Place {
+  int lane, warp, rank, b, c0;
+  bool active;
+  int64_t state;                                 // of the lane's first channel in a (sequences, D) tensor's row b
+  __device__ explicit Place(const ScanParams& p) {
+    lane = threadIdx.x & 31;
+    warp = threadIdx.x >> 5;
+    rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int unit = blockIdx.x / p.cluster, slice = unit % p.slices;
+    b = unit / p.slices;
+    c0 = (slice * 32 + lane) * VEC;
+    active = c0 < p.D;
+    state = static_cast<int64_t>(b) * p.D + c0;
+  }
+};
+
+// A run's map from zero, its rows already with the states that documents bring.  CUTS: a document opens or closes in the run; the warps
+// that hold none (documents are longer than sixteen tokens as a rule) do without the selections.
+template <bool CUTS, int VEC>
+__device__ __forceinline__ void run_forward(const RowDocs& docs, const Lanes<VEC> (&a)[SCAN_ROWS], const Lanes<VEC> (&x)[SCAN_ROWS], Lanes<VEC>& A,
+                                            Lanes<VEC>& H) {
+#pragma unroll
+  for (int r = 0; r < SCAN_ROWS; ++r) {
+    H = CUTS && docs.starts_at(r) ? x[r] : fma(a[r], H, x[r]);
+    A = mul(A, a[r]);
+  }
+}
+// lam of row r from the one behind it; where a document ends in the row nothing comes from behind.
+template <bool CUTS, int VEC>
+__device__ __forceinline__ void run_reverse(const RowDocs& docs, const Lanes<VEC> (&a)[SCAN_ROWS], const Lanes<VEC> (&dh)[SCAN_ROWS], Lanes<VEC>& M) {
+  Lanes<VEC> lam = dh[SCAN_ROWS - 1];
+#pragma unroll
+  for (int r = SCAN_ROWS - 2; r >= 0; --r) lam = CUTS && docs.ends_at(r) ? dh[r] : fma(a[r + 1], lam, dh[r]);
+  M = mul(a[0], lam);
+}
+// The documents that open in a run bring their own states in with their first tokens.
+template <int VEC>
+__device__ __forceinline__ void bring_states(const ScanParams& p, const RowDocs& docs, int c0, bool active, const Lanes<VEC> (&a)[SCAN_ROWS],
+                                             Lanes<VEC> (&x)[SCAN_ROWS]) {
+#pragma unroll
+  for (int r = 0; r < SCAN_ROWS; ++r)
+    if (docs.starts_at(r)) x[r] = fma(a[r], load_f32<VEC>(p.initial + static_cast<int64_t>(docs.opened(r)) * p.D + c0, active), x[r]);
 }
 
 template <typename TX, typename TG, int VEC, bool PACKED>
-__global__ void __launch_bounds__(32 * SCAN_WARPS)
+__global__ void __launch_bounds__(32 * SCAN_WARPS, sizeof(TX) == 2 ? 2 : 1)
 scan_fwd_kernel(ScanParams p) {
-  __shared__ WarpMaps<VEC, 2> maps;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int slice = blockIdx.x % p.slices, b = blockIdx.x / p.slices;
-  const int c0 = (slice * 32 + lane) * VEC;
-  const bool active = c0 < p.D;
-  const int64_t xb = b * p.x.sb + c0, gb = b * p.g.sb + c0;
-  float carry[VEC];                              // the state before the tile, the same in every warp
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    carry[i] = !PACKED && p.initial && active ? p.initial[static_cast<int64_t>(b) * p.D + c0 + i] : 0.f;
+  using MapT = Map<VEC, PACKED>;
+  __shared__ SharedMaps<VEC, SCAN_WARPS, PACKED> maps;
+  __shared__ SharedMaps<VEC, SCAN_MAX_CLUSTER, PACKED> blocks;
+  const Place<VEC> at(p);
+  const int lane = at.lane, warp = at.warp, c0 = at.c0;
+  const bool active = at.active;
+  const int64_t xb = at.b * p.x.sb + (active ? c0 : 0), gb = at.b * p.g.sb + (active ? c0 : 0);
+  // the state before the round's tiles, the same in every warp of the cluster
+  Lanes<VEC> carry = load_f32<VEC>(p.initial + at.state, !PACKED && p.initial && active);
 
-  for (int tile = 0; tile < p.tiles; ++tile) {
-    const int t0 = tile * SCAN_TILE + warp * SCAN_ROWS, buf = tile & 1;
-    float a[SCAN_ROWS][VEC], x[SCAN_ROWS][VEC];
-    load_rows<TX, VEC>(p.x, xb, t0, p.T, active, x);
-    load_rows<TG, VEC>(p.g, gb, t0, p.T, active, a);
-    const RowDocs docs = row_docs<PACKED>(p, t0, lane);
-    float A[VEC], H[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) A[i] = 1.f, H[i] = 0.f;
-#pragma unroll
-    for (int r = 0; r < SCAN_ROWS; ++r) {
-      const bool starts = PACKED && (docs.starts >> r & 1);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) a[r][i] = decay(a[r][i]);
-      if (PACKED && starts && p.initial) {       // the document's own state comes in with its first token
-        const int64_t at = static_cast<int64_t>(docs.opened(r)) * p.D + c0;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[r][i] = fmaf(a[r][i], active ? p.initial[at + i] : 0.f, x[r][i]);
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        H[i] = starts ? x[r][i] : fmaf(a[r][i], H[i], x[r][i]);
-        A[i] *= a[r][i];
-      }
+  RawRows<TX, VEC> xr;
+  RawRows<TG, VEC> gr;
+  request_rows<TX, VEC>(p.x, xb, at.rank * SCAN_TILE + warp * SCAN_ROWS, p.T, xr);
+  request_rows<TG, VEC>(p.g, gb, at.rank * SCAN_TILE + warp * SCAN_ROWS, p.T, gr);
+  for (int round = 0; round * p.cluster < p.tiles; ++round) {
+    const int tile = round * p.cluster + at.rank, t0 = tile * SCAN_TILE + warp * SCAN_ROWS, buf = round & 1;
+    Lanes<VEC> a[SCAN_ROWS], x[SCAN_ROWS];
+    unpack_rows<TX, VEC>(xr, x);
+    unpack_rows<TG, VEC>(gr, a);
+    if ((round + 1) * p.cluster < p.tiles) {
+      request_rows<TX, VEC>(p.x, xb, t0 + p.cluster * SCAN_TILE, p.T, xr);
+      request_rows<TG, VEC>(p.g, gb, t0 + p.cluster * SCAN_TILE, p.T, gr);
     }
-    write_map<VEC>(maps.v[buf][0][warp], lane, A);
-    write_map<VEC>(maps.v[buf][1][warp], lane, H);
-    if (PACKED && lane == 0) maps.cut[buf][0][warp] = docs.starts != 0;
+    const RowDocs docs = row_docs<PACKED>(p, t0, lane);
+    const bool cuts = PACKED && docs.any();
+    decays<VEC>(a);
+    MapT run = MapT::identity();
+    if (cuts) {
+      if (p.initial) bring_states<VEC>(p, docs, c0, active, a, x);
+      run.cut = docs.starts != 0;
+      run_forward<true, VEC>(docs, a, x, run.A, run.H);
+    } else {
+      run_forward<false, VEC>(docs, a, x, run.A, run.H);
+    }
+    maps.put(buf, warp, lane, run);
     __syncthreads();
 
-    // the map of the warps before this one, then of all, each applied to the state before the tile
-    float mine[VEC], pa[VEC], ph[VEC];
-    bool cut = false;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) pa[i] = 1.f, ph[i] = 0.f, mine[i] = carry[i];
-    if (p.carry && warp == 0 && active) {
-      float* at = p.carry + (static_cast<int64_t>(b) * p.tiles + tile) * p.D + c0;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) at[i] = carry[i];
-    }
-#pragma unroll
-    for (int w = 0; w < SCAN_WARPS; ++w) {
-      const Channels<VEC> wa = read_map<VEC>(maps.v[buf][0][w], lane), wh = read_map<VEC>(maps.v[buf][1][w], lane);
-      const bool wcut = PACKED && maps.cut[buf][0][w];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (w == warp) mine[i] = cut ? ph[i] : fmaf(pa[i], carry[i], ph[i]);
-        ph[i] = wcut ? wh.v[i] : fmaf(wa.v[i], ph[i], wh.v[i]);
-        pa[i] *= wa.v[i];
+    // the maps of the warps before this one, and of all of the block; then the state before the tile
+    MapT whole = MapT::identity();
+#pragma unroll 2
+    for (int w = 0; w < warp; ++w) whole.then(maps.get(buf, w, lane));
+    const MapT before = whole;
+#pragma unroll 2
+    for (int w = warp; w < SCAN_WARPS; ++w) whole.then(maps.get(buf, w, lane));
+    Lanes<VEC> mine = carry;
+    if (p.cluster > 1) {
+      put_in_cluster<VEC, PACKED>(blocks, buf, at.rank, p.cluster, warp, lane, whole);
+      cluster_arrive();
+      cluster_wait();
+      for (int k = 0; k < p.cluster; ++k) {
+        if (k == at.rank) mine = carry;
+        blocks.get(buf, k, lane).apply(carry);
       }
-      cut = cut || wcut;
+    } else {
+      whole.apply(carry);
     }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) carry[i] = cut ? ph[i] : fmaf(pa[i], carry[i], ph[i]);
+    if (p.carry && warp == 0 && active && tile < p.tiles) store_f32<VEC>(p.carry + (static_cast<int64_t>(at.b) * p.tiles + tile) * p.D + c0, mine);
+    before.apply(mine);
 
-    TX* out = static_cast<TX*>(p.h) + (static_cast<int64_t>(b) * p.T + t0) * p.D + c0;
+    TX* out = static_cast<TX*>(p.h) + (static_cast<int64_t>(at.b) * p.T + t0) * p.D + c0;
+    const int rows = active ? p.T - t0 : 0, stride = opaque(p.D);
+    if (cuts) {
 #pragma unroll
-    for (int r = 0; r < SCAN_ROWS; ++r) {
+      for (int r = 0; r < SCAN_ROWS; ++r) {
+        mine = docs.starts_at(r) ? x[r] : fma(a[r], mine, x[r]);
+        if (r < rows) store_pack<TX, VEC>(row_of(out, r, stride), mine.v);
+        if (p.final_state && docs.ends_at(r)) {
+          const int doc = docs.closed(r);
+          if (active && doc >= 0) store_f32<VEC>(p.final_state + static_cast<int64_t>(doc) * p.D + c0, mine);
+        }
+      }
+    } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) mine[i] = PACKED && (docs.starts >> r & 1) ? x[r][i] : fmaf(a[r][i], mine[i], x[r][i]);
-      if (active && t0 + r < p.T) store_pack<TX, VEC>(out + static_cast<int64_t>(r) * p.D, mine);
-      if (PACKED && p.final_state && (docs.ends >> r & 1)) {
-        const int doc = docs.closed(r);
-        if (active && doc >= 0)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) p.final_state[static_cast<int64_t>(doc) * p.D + c0 + i] = mine[i];
+      for (int r = 0; r < SCAN_ROWS; ++r) {
+        mine = fma(a[r], mine, x[r]);
+        if (r < rows) store_pack<TX, VEC>(row_of(out, r, stride), mine.v);
       }
     }
   }
   // Rows past T are identity maps (a = 1, x = 0), so the state behind the last tile is the one after the last token.
-  if (!PACKED && p.final_state && warp == 0 && active)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) p.final_state[static_cast<int64_t>(b) * p.D + c0 + i] = carry[i];
+  if (!PACKED && p.final_state && warp == 0 && at.rank == 0 && active) store_f32<VEC>(p.final_state + at.state, carry);
 }
 
 template <typename TX, typename TG, int VEC, bool PACKED>
 __global__ void __launch_bounds__(32 * SCAN_WARPS)
 scan_bwd_kernel(ScanParams p) {
-  __shared__ WarpMaps<VEC, 3> maps;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int slice = blockIdx.x % p.slices, b = blockIdx.x / p.slices;
-  const int c0 = (slice * 32 + lane) * VEC;
-  const bool active = c0 < p.D;
-  const int64_t xb = b * p.x.sb + c0, gb = b * p.g.sb + c0, hb = b * p.dh.sb + c0;
-  float carry[VEC];                              // mu behind the tile, the same in every warp
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) carry[i] = !PACKED && p.dfinal && active ? p.dfinal[static_cast<int64_t>(b) * p.D + c0 + i] : 0.f;
+  using MapT = Map<VEC, PACKED>;
+  __shared__ SharedMaps<VEC, SCAN_WARPS, PACKED> maps, reverse_maps;
+  __shared__ SharedMaps<VEC, SCAN_MAX_CLUSTER, PACKED> blocks;
+  const Place<VEC> at(p);
+  const int lane = at.lane, warp = at.warp, c0 = at.c0;
+  const bool active = at.active;
+  const int64_t xb = at.b * p.x.sb + (active ? c0 : 0), gb = at.b * p.g.sb + (active ? c0 : 0), hb = at.b * p.dh.sb + (active ? c0 : 0);
+  // mu behind the round's tiles, the same in every warp of the cluster
+  Lanes<VEC> carry = load_f32<VEC>(p.dfinal + at.state, !PACKED && p.dfinal && active);
 
-  for (int tile = p.tiles - 1; tile >= 0; --tile) {
-    const int t0 = tile * SCAN_TILE + warp * SCAN_ROWS, buf = tile & 1;
-    float a[SCAN_ROWS][VEC], x[SCAN_ROWS][VEC], dh[SCAN_ROWS][VEC];
-    load_rows<TX, VEC>(p.x, xb, t0, p.T, active, x);
-    load_rows<TG, VEC>(p.g, gb, t0, p.T, active, a);
-    load_rows<TX, VEC>(p.dh, hb, t0, p.T, active, dh);
+  const int rounds = (p.tiles + p.cluster - 1) / p.cluster;
+  RawRows<TX, VEC> xr, hr;
+  RawRows<TG, VEC> gr;
+  auto request = [&](int t0) {
+    request_rows<TX, VEC>(p.x, xb, t0, p.T, xr);
+    request_rows<TG, VEC>(p.g, gb, t0, p.T, gr);
+    request_rows<TX, VEC>(p.dh, hb, t0, p.T, hr);
+  };
+  request(((rounds - 1) * p.cluster + at.rank) * SCAN_TILE + warp * SCAN_ROWS);
+  for (int round = rounds - 1; round >= 0; --round) {
+    const int tile = round * p.cluster + at.rank, t0 = tile * SCAN_TILE + warp * SCAN_ROWS, buf = round & 1;
+    Lanes<VEC> a[SCAN_ROWS], x[SCAN_ROWS], dh[SCAN_ROWS];
+    unpack_rows<TX, VEC>(xr, x);
+    unpack_rows<TG, VEC>(gr, a);
+    unpack_rows<TX, VEC>(hr, dh);
+    if (round > 0) request(t0 - p.cluster * SCAN_TILE);
     const RowDocs docs = row_docs<PACKED>(p, t0, lane);
-    float h[VEC];                                // the state before the tile
+    const bool cuts = PACKED && docs.any();
+    // the state before the tile
+    Lanes<VEC> h = load_f32<VEC>(p.carry + (static_cast<int64_t>(at.b) * p.tiles + tile) * p.D + c0, active && tile < p.tiles);
+    decays<VEC>(a);
+    MapT run = MapT::identity(), back = run;
+    if (cuts) {
+      if (p.initial) bring_states<VEC>(p, docs, c0, active, a, x);
+      if (p.dfinal) {                            // the gradient of a final state comes in with its document's last token
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) h[i] = active ? p.carry[(static_cast<int64_t>(b) * p.tiles + tile) * p.D + c0 + i] : 0.f;
-    float A[VEC], H[VEC], M[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) A[i] = 1.f, H[i] = 0.f, M[i] = 0.f;
-#pragma unroll
-    for (int r = 0; r < SCAN_ROWS; ++r) {
-      const bool starts = PACKED && (docs.starts >> r & 1);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) a[r][i] = decay(a[r][i]);
-      if (PACKED && starts && p.initial) {
-        const int64_t at = static_cast<int64_t>(docs.opened(r)) * p.D + c0;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[r][i] = fmaf(a[r][i], active ? p.initial[at + i] : 0.f, x[r][i]);
+        for (int r = 0; r < SCAN_ROWS; ++r)
+          if (docs.ends_at(r)) {
+            const int doc = docs.closed(r);
+            dh[r] = add(dh[r], load_f32<VEC>(p.dfinal + static_cast<int64_t>(doc) * p.D + c0, active && doc >= 0));
+          }
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        H[i] = starts ? x[r][i] : fmaf(a[r][i], H[i], x[r][i]);
-        A[i] *= a[r][i];
-      }
-      if (PACKED && p.dfinal && (docs.ends >> r & 1)) {      // the gradient of a final state comes in with the last token
-        const int doc = docs.closed(r);
-        if (active && doc >= 0)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) dh[r][i] += p.dfinal[static_cast<int64_t>(doc) * p.D + c0 + i];
-      }
+      run.cut = docs.starts != 0;
+      back.cut = docs.ends != 0;
+      run_forward<true, VEC>(docs, a, x, run.A, run.H);
+      run_reverse<true, VEC>(docs, a, dh, back.H);
+    } else {
+      run_forward<false, VEC>(docs, a, x, run.A, run.H);
+      run_reverse<false, VEC>(docs, a, dh, back.H);
     }
-#pragma unroll
-    for (int r = SCAN_ROWS - 1; r >= 0; --r)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) M[i] = a[r][i] * (PACKED && (docs.ends >> r & 1) ? dh[r][i] : dh[r][i] + M[i]);
-    write_map<VEC>(maps.v[buf][0][warp], lane, A);
-    write_map<VEC>(maps.v[buf][1][warp], lane, H);
-    write_map<VEC>(maps.v[buf][2][warp], lane, M);
-    if (PACKED && lane == 0) maps.cut[buf][0][warp] = docs.starts != 0, maps.cut[buf][1][warp] = docs.ends != 0;
+    back.A = run.A;
+    maps.put(buf, warp, lane, run);
+    reverse_maps.put(buf, warp, lane, back);
     __syncthreads();
 
-    float pa[VEC], ph[VEC], mu[VEC];
-    bool cut = false;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) pa[i] = 1.f, ph[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < SCAN_WARPS; ++w) {
-      if (w == warp) break;
-      const Channels<VEC> wa = read_map<VEC>(maps.v[buf][0][w], lane), wh = read_map<VEC>(maps.v[buf][1][w], lane);
-      const bool wcut = PACKED && maps.cut[buf][0][w];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        ph[i] = wcut ? wh.v[i] : fmaf(wa.v[i], ph[i], wh.v[i]);
-        pa[i] *= wa.v[i];
-      }
-      cut = cut || wcut;
+    MapT whole = MapT::identity();
+#pragma unroll 2
+    for (int w = SCAN_WARPS - 1; w > warp; --w) whole.then(reverse_maps.get(buf, w, lane));
+    const MapT behind = whole;
+#pragma unroll 2
+    for (int w = warp; w >= 0; --w) whole.then(reverse_maps.get(buf, w, lane));
+    if (p.cluster > 1) {
+      put_in_cluster<VEC, PACKED>(blocks, buf, at.rank, p.cluster, warp, lane, whole);
+      cluster_arrive();
     }
+    MapT before = MapT::identity();
+#pragma unroll 2
+    for (int w = 0; w < warp; ++w) before.then(maps.get(buf, w, lane));
+    before.apply(h);
+    if (cuts) {                                  // x becomes the state before its row
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) h[i] = cut ? ph[i] : fmaf(pa[i], h[i], ph[i]);
-    cut = false;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) pa[i] = 1.f, ph[i] = 0.f, mu[i] = carry[i];
-#pragma unroll
-    for (int w = SCAN_WARPS - 1; w >= 0; --w) {
-      const Channels<VEC> wa = read_map<VEC>(maps.v[buf][0][w], lane), wm = read_map<VEC>(maps.v[buf][2][w], lane);
-      const bool wcut = PACKED && maps.cut[buf][1][w];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (w == warp) mu[i] = cut ? ph[i] : fmaf(pa[i], carry[i], ph[i]);
-        ph[i] = wcut ? wm.v[i] : fmaf(wa.v[i], ph[i], wm.v[i]);
-        pa[i] *= wa.v[i];
+      for (int r = 0; r < SCAN_ROWS; ++r) {
+        Lanes<VEC> last = h;
+        if (docs.starts_at(r))
+          last = p.initial ? load_f32<VEC>(p.initial + static_cast<int64_t>(docs.opened(r)) * p.D + c0, active) : all<VEC>(0.f);
+        h = docs.starts_at(r) ? x[r] : fma(a[r], h, x[r]);
+        x[r] = last;
       }
-      cut = cut || wcut;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) carry[i] = cut ? ph[i] : fmaf(pa[i], carry[i], ph[i]);
+      for (int r = 0; r < SCAN_ROWS; ++r) {
+        const Lanes<VEC> last = h;
+        h = fma(a[r], h, x[r]);
+        x[r] = last;
+      }
+    }
+    Lanes<VEC> mu = carry;
+    if (p.cluster > 1) {
+      cluster_wait();
+      for (int k = p.cluster - 1; k >= 0; --k) {
+        if (k == at.rank) mu = carry;
+        blocks.get(buf, k, lane).apply(carry);
+      }
+    } else {
+      whole.apply(carry);
+    }
+    behind.apply(mu);
 
-#pragma unroll
-    for (int r = 0; r < SCAN_ROWS; ++r) {        // x becomes the state before its row
-      const bool starts = PACKED && (docs.starts >> r & 1);
-      float own[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) own[i] = 0.f;
-      if (PACKED && starts && p.initial) {
-        const int64_t at = static_cast<int64_t>(docs.opened(r)) * p.D + c0;
-        if (active)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) own[i] = p.initial[at + i];
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float before = starts ? own[i] : h[i];
-        h[i] = starts ? x[r][i] : fmaf(a[r][i], h[i], x[r][i]);
-        x[r][i] = before;
-      }
-    }
-    const int64_t row = (static_cast<int64_t>(b) * p.T + t0) * p.D + c0;
+    const int64_t row = (static_cast<int64_t>(at.b) * p.T + t0) * p.D + c0;
     TX* dx = static_cast<TX*>(p.dx) + row;
     TG* dg = static_cast<TG*>(p.dg) + row;
+    const int rows = active ? p.T - t0 : 0, stride = opaque(p.D);
+    Lanes<VEC> lam = cuts && docs.ends_at(SCAN_ROWS - 1) ? dh[SCAN_ROWS - 1] : add(dh[SCAN_ROWS - 1], mu);
 #pragma unroll
     for (int r = SCAN_ROWS - 1; r >= 0; --r) {
-      float lam[VEC], d[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        lam[i] = PACKED && (docs.ends >> r & 1) ? dh[r][i] : dh[r][i] + mu[i];
-        mu[i] = a[r][i] * lam[i];
-        d[i] = mu[i] * x[r][i];
+      if (r < SCAN_ROWS - 1) lam = cuts && docs.ends_at(r) ? dh[r] : fma(a[r + 1], lam, dh[r]);
+      mu = mul(a[r], lam);
+      const Lanes<VEC> d = mul(mu, x[r]);
+      if (r < rows) {
+        store_pack<TX, VEC>(row_of(dx, r, stride), lam.v);
+        store_pack<TG, VEC>(row_of(dg, r, stride), d.v);
       }
-      if (active && t0 + r < p.T) {
-        store_pack<TX, VEC>(dx + static_cast<int64_t>(r) * p.D, lam);
-        store_pack<TG, VEC>(dg + static_cast<int64_t>(r) * p.D, d);
-      }
-      if (PACKED && p.dinitial && (docs.starts >> r & 1)) {
+      if (cuts && p.dinitial && docs.starts_at(r)) {
         const int doc = docs.opened(r);
-        if (active)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) p.dinitial[static_cast<int64_t>(doc) * p.D + c0 + i] = mu[i];
+        if (active) store_f32<VEC>(p.dinitial + static_cast<int64_t>(doc) * p.D + c0, mu);
       }
     }
   }
-  if (!PACKED && p.dinitial && warp == 0 && active)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) p.dinitial[static_cast<int64_t>(b) * p.D + c0 + i] = carry[i];
+  if (!PACKED && p.dinitial && warp == 0 && at.rank == 0 && active) store_f32<VEC>(p.dinitial + at.state, carry);
 }
 
 // One token: state <- exp(g) state + x in place, h the new state in x's type.  A stream over the state.
@@ -364,7 +528,7 @@ scan_step_kernel(const TX* x, int64_t x_row, const TG* g, int64_t g_row, float* 
   const Pack<float, VEC> s = load_pack<float, VEC>(state + b * D + c);
   float v[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) v[k] = fmaf(decay(to_f32(gv.v[k])), s.v[k], to_f32(xv.v[k]));
+  for (int k = 0; k < VEC; ++k) v[k] = fmaf(decay<1>(Lanes<1>{{to_f32(gv.v[k])}}).v[0], s.v[k], to_f32(xv.v[k]));
   store_pack<float, VEC>(state + b * D + c, v);
   store_pack<TX, VEC>(h + b * D + c, v);
 }
@@ -400,11 +564,22 @@ namespace {
 template <bool BACKWARD, typename TX, typename TG, int VEC, bool PACKED>
 int launch_scan(ScanParams p, cudaStream_t s) {
   p.slices = (p.D + 32 * VEC - 1) / (32 * VEC);
-  const int64_t blocks = static_cast<int64_t>(p.B) * p.slices;
-  if (blocks > 0x7fffffffLL) return TGDN_ERR_SHAPE;
-  if constexpr (BACKWARD) scan_bwd_kernel<TX, TG, VEC, PACKED><<<static_cast<unsigned>(blocks), 32 * SCAN_WARPS, 0, s>>>(p);
-  else scan_fwd_kernel<TX, TG, VEC, PACKED><<<static_cast<unsigned>(blocks), 32 * SCAN_WARPS, 0, s>>>(p);
-  return tgdn_cuda_error(cudaGetLastError());
+  const int64_t units = static_cast<int64_t>(p.B) * p.slices;
+  p.cluster = 1;
+  while (p.cluster < SCAN_MAX_CLUSTER && p.cluster < p.tiles && units * p.cluster * 2 <= tgdn_sm_count()) p.cluster *= 2;
+  if (units * p.cluster > 0x7fffffffLL) return TGDN_ERR_SHAPE;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(units * p.cluster));
+  config.blockDim = dim3(32 * SCAN_WARPS);
+  config.stream = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(p.cluster);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = p.cluster > 1 ? 1 : 0;
+  if constexpr (BACKWARD) return tgdn_cuda_error(cudaLaunchKernelEx(&config, scan_bwd_kernel<TX, TG, VEC, PACKED>, p));
+  else return tgdn_cuda_error(cudaLaunchKernelEx(&config, scan_fwd_kernel<TX, TG, VEC, PACKED>, p));
 }
 
 template <bool BACKWARD, typename TX, typename TG>
@@ -423,12 +598,15 @@ int launch_scan_any(const ScanParams& p, int xt, int gt, bool pairs, cudaStream_
   return TGDN_ERR_TYPE;
 }
 
+ScanIn scan_in(const tgdn_rows& t) { return {t.data, t.stride_outer, static_cast<int>(t.stride_inner)}; }
+
 bool in_pairs(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % (2 * type_bytes(type)) == 0; }
 
 int scan_checks(const tgdn_rows* x, const tgdn_rows* g, const int32_t* map, int n_docs, int B, int T, int D) {
   if (!x || !g || !x->data || !g->data) return TGDN_ERR_NULL;
-  if (B <= 0 || T <= 0 || D <= 0 || (map && (B != 1 || n_docs <= 0))) return TGDN_ERR_SHAPE;
+  if (B <= 0 || T <= 0 || T > 0x7fffffff - 2 * SCAN_MAX_CLUSTER * SCAN_TILE || D <= 0 || (map && (B != 1 || n_docs <= 0))) return TGDN_ERR_SHAPE;
   if (!type_known(x->type) || !type_known(g->type)) return TGDN_ERR_TYPE;
+  if (x->stride_inner > 0x7fffffffLL || g->stride_inner > 0x7fffffffLL || x->stride_inner < 0 || g->stride_inner < 0) return TGDN_ERR_SHAPE;
   return 0;
 }
 
@@ -452,8 +630,8 @@ extern "C" int tgdn_scan_fwd(const tgdn_rows* host_x, const tgdn_rows* host_g, c
   if (!h) return TGDN_ERR_NULL;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   ScanParams p{};
-  p.x = {host_x->data, host_x->stride_outer, host_x->stride_inner};
-  p.g = {host_g->data, host_g->stride_outer, host_g->stride_inner};
+  p.x = scan_in(*host_x);
+  p.g = scan_in(*host_g);
   p.map = map; p.initial = initial; p.h = h; p.final_state = final_state; p.carry = carry;
   p.B = B; p.T = T; p.D = D; p.n_docs = n_docs;
   p.tiles = (T - 1) / SCAN_TILE + 1;
@@ -467,11 +645,12 @@ extern "C" int tgdn_scan_bwd(const tgdn_rows* host_x, const tgdn_rows* host_g, c
   if (const int rc = scan_checks(host_x, host_g, map, n_docs, B, T, D)) return rc;
   if (!host_dh || !host_dh->data || !carry || !dx || !dg) return TGDN_ERR_NULL;
   if (host_dh->type != host_x->type) return TGDN_ERR_TYPE;
+  if (host_dh->stride_inner > 0x7fffffffLL || host_dh->stride_inner < 0) return TGDN_ERR_SHAPE;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   ScanParams p{};
-  p.x = {host_x->data, host_x->stride_outer, host_x->stride_inner};
-  p.g = {host_g->data, host_g->stride_outer, host_g->stride_inner};
-  p.dh = {host_dh->data, host_dh->stride_outer, host_dh->stride_inner};
+  p.x = scan_in(*host_x);
+  p.g = scan_in(*host_g);
+  p.dh = scan_in(*host_dh);
   p.map = map; p.initial = initial; p.carry = const_cast<float*>(carry); p.dfinal = dfinal;
   p.dx = dx; p.dg = dg; p.dinitial = dinitial;
   p.B = B; p.T = T; p.D = D; p.n_docs = n_docs;
