@@ -127,17 +127,23 @@ int tgdn_make_gate_map(CUtensorMap* map, const float* base, int B, int T, int H,
 
 int tgdn_make_rows_map(CUtensorMap* map, const void* base, int C, int T, int B, int64_t stride_t, int64_t stride_b, int box_cols,
                        int box_rows) {
+  return tgdn_make_typed_rows_map(map, base, TGDN_BF16, C, T, B, stride_t, stride_b, box_cols, box_rows);
+}
+
+int tgdn_make_typed_rows_map(CUtensorMap* map, const void* base, int type, int C, int T, int B, int64_t stride_t, int64_t stride_b,
+                             int box_cols, int box_rows) {
   EncodeTiledFn fn = encode_tiled();
   if (!fn) return TGDN_ERR_DRIVER;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || (stride_t % 8) || (stride_b % 8)) return TGDN_ERR_ALIGN;
+  const int size = type == TGDN_F32 ? 4 : 2, piece = 16 / size;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (stride_t % piece) || (stride_b % piece)) return TGDN_ERR_ALIGN;
   if (box_cols > 256 || box_rows > 256) return TGDN_ERR_SHAPE;
   // a single batch row needs no third stride; give it any valid multiple of 16 bytes
-  const cuuint64_t sb = (B > 1) ? static_cast<cuuint64_t>(stride_b) * 2 : static_cast<cuuint64_t>(stride_t) * 2 * static_cast<cuuint64_t>(T);
+  const cuuint64_t row = static_cast<cuuint64_t>(stride_t) * size, sb = B > 1 ? static_cast<cuuint64_t>(stride_b) * size : row * static_cast<cuuint64_t>(T);
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(C), static_cast<cuuint64_t>(T), static_cast<cuuint64_t>(B)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride_t) * 2, sb};
+  const cuuint64_t strides[2] = {row, sb};
   const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+  CUresult r = fn(map, type == TGDN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == TGDN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : TGDN_ERR_DRIVER;

@@ -34,6 +34,9 @@ int tgdn_make_gate_map(CUtensorMap* map, const float* base, int B, int T, int H,
 // Tensor map over a (B, T, C) bf16 tensor with element strides (stride_b, stride_t, 1): box = [box_cols][box_rows][1], no swizzle.
 int tgdn_make_rows_map(CUtensorMap* map, const void* base, int C, int T, int B, int64_t stride_t, int64_t stride_b, int box_cols,
                        int box_rows);
+// The same for elements of any of the types TGDN_F32, TGDN_BF16, TGDN_F16.
+int tgdn_make_typed_rows_map(CUtensorMap* map, const void* base, int type, int C, int T, int B, int64_t stride_t, int64_t stride_b,
+                             int box_cols, int box_rows);
 
 // True when the current device is compute capability 10.x; also binds the device's primary context to the calling thread.
 int tgdn_check_device();

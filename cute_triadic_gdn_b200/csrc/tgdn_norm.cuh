@@ -21,6 +21,7 @@
 
 #include "tgdn_common.cuh"
 #include "tgdn_host.h"
+#include "tgdn_kernels.h"
 #include "tgdn_rows.cuh"
 
 namespace tgdn {

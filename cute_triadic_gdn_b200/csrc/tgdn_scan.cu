@@ -14,8 +14,11 @@
 //
 // Sums, products and states are f32.  Maps are composed in an order given by the tile alone, so a sequence's results do not depend on
 // what runs beside it.
+#include <type_traits>
+
 #include "tgdn_common.cuh"
 #include "tgdn_host.h"
+#include "tgdn_kernels.h"
 #include "tgdn_rows.cuh"
 
 namespace tgdn {
@@ -43,7 +46,8 @@ struct ScanParams {
   void* dx;
   void* dg;
   float* dinitial;
-  int B, T, D, n_docs, slices, tiles, cluster;
+  int B, T, D, n_docs, slices, tiles, cluster, stages;
+  int* status;
 };
 
 // A lane's channels of one row.  Pairs go through the two-wide f32 instructions: the kernels would be bound by the issue of
@@ -129,13 +133,17 @@ struct RowDocs {
   __device__ int closed(int r) const { return __shfl_sync(0xffffffffu, code, r + 1) - 2; }
 };
 
+// The lane's entry of the map for the rows from t0 on (and the one behind them): asked for a round ahead.
 template <bool PACKED>
-__device__ __forceinline__ RowDocs row_docs(const ScanParams& p, int t0, int lane) {
-  RowDocs d{0u, 0u, 0};
+__device__ __forceinline__ int row_code(const ScanParams& p, int t0, int lane) {
+  const int t = t0 + lane;
+  return !PACKED || lane > SCAN_ROWS || t > p.T ? 0 : t == p.T ? p.n_docs + 1 : p.map[t];
+}
+template <bool PACKED>
+__device__ __forceinline__ RowDocs row_docs(const ScanParams& p, int t0, int code) {
+  RowDocs d{0u, 0u, code};
   if constexpr (PACKED) {
-    const int t = t0 + lane;
-    if (lane <= SCAN_ROWS) d.code = t < p.T ? p.map[t] : t == p.T ? p.n_docs + 1 : 0;
-    const uint32_t b = __ballot_sync(0xffffffffu, d.code != 0);
+    const uint32_t b = __ballot_sync(0xffffffffu, code != 0);
     d.starts = b & ((1u << SCAN_ROWS) - 1);
     if (t0 + SCAN_ROWS > p.T && t0 <= p.T) d.starts &= (1u << (p.T - t0)) - 1;
     d.ends = (b >> 1) & ((1u << SCAN_ROWS) - 1);
@@ -232,36 +240,127 @@ __device__ __forceinline__ uint32_t in_block_of_cluster(const void* p, uint32_t 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
-__device__ __forceinline__ void put_remote(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
-__device__ __forceinline__ void put_remote(uint32_t at, float v, float w) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v), "f"(w) : "memory");
+// Stores into another block's shared memory that count towards the barrier there with their bytes.
+__device__ __forceinline__ void send(uint32_t at, uint32_t bar, uint32_t v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(at), "r"(v), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void put_remote(uint32_t at, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
-// The hardware's barrier over the blocks of a cluster, which all take every one: what was written before it is seen behind it.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void send(uint32_t at, uint32_t bar, float v, float w) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(at), "f"(v), "f"(w), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void send(uint32_t at, uint32_t bar, float a, float b, float c, float d) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(at), "f"(a), "f"(b), "f"(c), "f"(d), "r"(bar) : "memory");
+}
+// The hardware's barrier over the blocks of a cluster, at the kernel's two ends.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
-// Leaves the block's map with every block of the cluster, warp k at the k-th.
+// The maps that the blocks of a cluster send one another, warp k of each to block k.  Two buffers by turns: a block sends its map of round
+// n + 2 when it has those of round n + 1, which their blocks sent behind a barrier of all their warps, done with round n.  Messages and a
+// barrier on their bytes instead of the cluster's own barrier: that one also waits for the output's stores on their way to memory, 4 us a
+// round (packed, 131072 x 1024).
 template <int VEC, bool PACKED>
-__device__ __forceinline__ void put_in_cluster(SharedMaps<VEC, SCAN_MAX_CLUSTER, PACKED>& at, int buf, int rank, int blocks, int warp, int lane,
-                                               const Map<VEC, PACKED>& m) {
-  for (int k = warp; k < blocks; k += SCAN_WARPS) {
-    const uint32_t a = in_block_of_cluster(&at.A[buf][rank][lane], k), h = in_block_of_cluster(&at.H[buf][rank][lane], k);
-    if constexpr (VEC == 2) {
-      put_remote(a, m.A.v[0], m.A.v[1]);
-      put_remote(h, m.H.v[0], m.H.v[1]);
-    } else {
-      put_remote(a, m.A.v[0]);
-      put_remote(h, m.H.v[0]);
-    }
-    if (PACKED && lane == 0) put_remote(in_block_of_cluster(&at.cut[buf][rank], k), m.cut);
+struct ClusterMaps {
+  struct alignas(8 * VEC) Entry { Lanes<VEC> A, H; };
+  Entry map[2][SCAN_MAX_CLUSTER][32];
+  int cut[2][SCAN_MAX_CLUSTER];
+  uint64_t full[2];
+  static constexpr int BYTES = 32 * sizeof(Entry) + (PACKED ? 4 : 0);          // of one message
+  __device__ void init() {
+    mbar_init(&full[0], 1);
+    mbar_init(&full[1], 1);
+    mbar_fence_init();
   }
+  // One thread of the block, once a round; messages may come before.
+  __device__ void expect(int buf, int blocks) { mbar_expect_tx(&full[buf], blocks * BYTES); }
+  __device__ void send_to(int block, int buf, int rank, int lane, const Map<VEC, PACKED>& m) {
+    const uint32_t at = in_block_of_cluster(&map[buf][rank][lane], block), bar = in_block_of_cluster(&full[buf], block);
+    if constexpr (VEC == 2) send(at, bar, m.A.v[0], m.A.v[1], m.H.v[0], m.H.v[1]);
+    else send(at, bar, m.A.v[0], m.H.v[0]);
+    if (PACKED && lane == 0) send(in_block_of_cluster(&cut[buf][rank], block), bar, static_cast<uint32_t>(m.cut));
+  }
+  __device__ void wait(int buf, int turn, const WaitCtl& ctl) { mbar_wait_parked(&full[buf], turn & 1, ctl, DEV_TIMEOUT_LOAD); }
+  __device__ Map<VEC, PACKED> get(int buf, int rank, int lane) const {
+    const Entry e = map[buf][rank][lane];
+    return {e.A, e.H, PACKED ? cut[buf][rank] : 0};
+  }
+};
+
+// The ring of tiles on their way: stages of shared memory that the copy engine fills, each a block's rows of all its inputs, with a barrier
+// that completes when a stage's bytes are in.  One thread asks for a stage again as soon as all warps have what they need of it.
+constexpr int SCAN_MAX_STAGES = 4;
+__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int c, int t, int b) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c), "r"(t), "r"(b)
+               : "memory");
+}
+struct ScanMaps {
+  CUtensorMap x, g, dh;
+};
+struct RingControl {
+  uint64_t full[SCAN_MAX_STAGES];
+  int abort;
+};
+template <typename TX, typename TG, bool BACKWARD>
+struct Ring {
+  static constexpr int X_BYTES = SCAN_TILE * 64 * sizeof(TX), G_BYTES = SCAN_TILE * 64 * sizeof(TG);
+  static constexpr int BYTES = X_BYTES * (BACKWARD ? 2 : 1) + G_BYTES;
+  const ScanMaps& maps;
+  uint8_t* data;
+  RingControl* control;
+  WaitCtl wait_ctl;
+  int c, b, stages;
+  int stage = 0, parity = 0;                     // of the tile that is read next
+  int ask = 0, asked = 0;                        // the stage that is asked for next, and how many were (the asking thread's)
+
+  __device__ Ring(const ScanMaps& m, uint8_t* smem, RingControl* ctl, int* status, int c_, int b_, int stages_)
+      : maps(m), data(smem), control(ctl), wait_ctl{&ctl->abort, status}, c(c_), b(b_), stages(stages_) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) mbar_init(&control->full[i], 1);
+      control->abort = 0;
+      mbar_fence_init();
+    }
+    __syncthreads();
+  }
+  __device__ void request(int t) {
+    uint8_t* dst = data + ask * BYTES;
+    uint64_t* bar = &control->full[ask];
+    mbar_expect_tx(bar, BYTES);
+    tma_tile(dst, &maps.x, bar, c, t, b);
+    tma_tile(dst + X_BYTES, &maps.g, bar, c, t, b);
+    if constexpr (BACKWARD) tma_tile(dst + X_BYTES + G_BYTES, &maps.dh, bar, c, t, b);
+    ask = ask + 1 == stages ? 0 : ask + 1;
+    ++asked;
+  }
+  __device__ const uint8_t* wait() const {
+    mbar_wait_parked(&control->full[stage], parity, wait_ctl, DEV_TIMEOUT_LOAD);
+    return data + stage * BYTES;
+  }
+  __device__ void advance() {
+    if (++stage == stages) stage = 0, parity ^= 1;
+  }
+  // After a wait that was given up: nothing more is asked for, and what was must have landed before the block's memory goes.
+  __device__ bool given_up() const { return *wait_ctl.abort != 0; }
+  __device__ void drain() const {
+    int none = 0;
+    const WaitCtl again{&none, wait_ctl.status};
+    for (int n = asked > stages ? asked - stages : 0; n < asked; ++n) mbar_wait_parked(&control->full[n % stages], n / stages & 1, again, DEV_TIMEOUT_LOAD);
+  }
+};
+// A warp's rows of a tile in the ring, as they lie there.
+template <typename T, int VEC>
+__device__ __forceinline__ void take_rows(const uint8_t* tile, int warp, int lane, RawRows<T, VEC>& raw) {
+  using Raw = typename RawOf<VEC * sizeof(T)>::type;
+  const Raw* p = reinterpret_cast<const Raw*>(tile) + warp * SCAN_ROWS * 32 + lane;
+#pragma unroll
+  for (int r = 0; r < SCAN_ROWS; ++r) raw.v[r] = p[r * 32];
 }
 
 // Where a block stands: its slice of channels, its batch row, its place in the cluster.
 template <int VEC>
 struct Place {
-  int lane, warp, rank, b, c0;
+  int lane, warp, rank, b, slice0, c0;
   bool active;
   int64_t state;                                 // of the lane's first channel in a (sequences, D) tensor's row b
   __device__ explicit Place(const ScanParams& p) {
@@ -270,7 +369,8 @@ struct Place {
     rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int unit = blockIdx.x / p.cluster, slice = unit % p.slices;
     b = unit / p.slices;
-    c0 = (slice * 32 + lane) * VEC;
+    slice0 = slice * 32 * VEC;
+    c0 = slice0 + lane * VEC;
     active = c0 < p.D;
     state = static_cast<int64_t>(b) * p.D + c0;
   }
@@ -304,12 +404,18 @@ __device__ __forceinline__ void bring_states(const ScanParams& p, const RowDocs&
     if (docs.starts_at(r)) x[r] = fma(a[r], load_f32<VEC>(p.initial + static_cast<int64_t>(docs.opened(r)) * p.D + c0, active), x[r]);
 }
 
-template <typename TX, typename TG, int VEC, bool PACKED>
+// RING: pairs of channels, tiles by the copy engine (rows of whole 16-byte pieces).  Otherwise single channels by plain loads of any
+// alignment, the next tile in registers.
+template <typename TX, typename TG, bool RING, bool PACKED>
 __global__ void __launch_bounds__(32 * SCAN_WARPS, sizeof(TX) == 2 ? 2 : 1)
-scan_fwd_kernel(ScanParams p) {
+scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
+  constexpr int VEC = RING ? 2 : 1;
   using MapT = Map<VEC, PACKED>;
+  using BlockMaps = ClusterMaps<VEC, PACKED>;
+  extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ SharedMaps<VEC, SCAN_WARPS, PACKED> maps;
-  __shared__ SharedMaps<VEC, SCAN_MAX_CLUSTER, PACKED> blocks;
+  __shared__ RingControl control;
+  BlockMaps& blocks = *reinterpret_cast<BlockMaps*>(dynamic + (RING ? p.stages * Ring<TX, TG, false>::BYTES : 0));
   const Place<VEC> at(p);
   const int lane = at.lane, warp = at.warp, c0 = at.c0;
   const bool active = at.active;
@@ -317,20 +423,39 @@ scan_fwd_kernel(ScanParams p) {
   // the state before the round's tiles, the same in every warp of the cluster
   Lanes<VEC> carry = load_f32<VEC>(p.initial + at.state, !PACKED && p.initial && active);
 
+  const int step = p.cluster * SCAN_TILE, rounds = (p.tiles + p.cluster - 1) / p.cluster, first = at.rank * SCAN_TILE;
+  Ring<TX, TG, false> ring(tensors, dynamic, &control, p.status, at.slice0, at.b, RING ? p.stages : 0);
+  const bool asks = RING && threadIdx.x == 0;
+  if (p.cluster > 1) {
+    if (threadIdx.x == 0) blocks.init();
+    cluster_barrier();                           // no block sends to another before that one can take it
+  }
   RawRows<TX, VEC> xr;
   RawRows<TG, VEC> gr;
-  request_rows<TX, VEC>(p.x, xb, at.rank * SCAN_TILE + warp * SCAN_ROWS, p.T, xr);
-  request_rows<TG, VEC>(p.g, gb, at.rank * SCAN_TILE + warp * SCAN_ROWS, p.T, gr);
-  for (int round = 0; round * p.cluster < p.tiles; ++round) {
+  if (asks)
+    for (int n = 0; n < p.stages && n < rounds; ++n) ring.request(first + n * step);
+  if (!RING) {
+    request_rows<TX, VEC>(p.x, xb, first + warp * SCAN_ROWS, p.T, xr);
+    request_rows<TG, VEC>(p.g, gb, first + warp * SCAN_ROWS, p.T, gr);
+  }
+  int code = row_code<PACKED>(p, first + warp * SCAN_ROWS, lane);
+  for (int round = 0; round < rounds; ++round) {
     const int tile = round * p.cluster + at.rank, t0 = tile * SCAN_TILE + warp * SCAN_ROWS, buf = round & 1;
     Lanes<VEC> a[SCAN_ROWS], x[SCAN_ROWS];
+    if (RING) {
+      const uint8_t* here = ring.wait();
+      take_rows<TX, VEC>(here, warp, lane, xr);
+      take_rows<TG, VEC>(here + ring.X_BYTES, warp, lane, gr);
+      ring.advance();
+    }
     unpack_rows<TX, VEC>(xr, x);
     unpack_rows<TG, VEC>(gr, a);
-    if ((round + 1) * p.cluster < p.tiles) {
-      request_rows<TX, VEC>(p.x, xb, t0 + p.cluster * SCAN_TILE, p.T, xr);
-      request_rows<TG, VEC>(p.g, gb, t0 + p.cluster * SCAN_TILE, p.T, gr);
+    if (!RING && round + 1 < rounds) {
+      request_rows<TX, VEC>(p.x, xb, t0 + step, p.T, xr);
+      request_rows<TG, VEC>(p.g, gb, t0 + step, p.T, gr);
     }
-    const RowDocs docs = row_docs<PACKED>(p, t0, lane);
+    const RowDocs docs = row_docs<PACKED>(p, t0, code);
+    if (round + 1 < rounds) code = row_code<PACKED>(p, t0 + step, lane);
     const bool cuts = PACKED && docs.any();
     decays<VEC>(a);
     MapT run = MapT::identity();
@@ -343,6 +468,7 @@ scan_fwd_kernel(ScanParams p) {
     }
     maps.put(buf, warp, lane, run);
     __syncthreads();
+    if (asks && round + p.stages < rounds && !ring.given_up()) ring.request(first + (round + p.stages) * step);   // every warp has its rows
 
     // the maps of the warps before this one, and of all of the block; then the state before the tile
     MapT whole = MapT::identity();
@@ -353,9 +479,9 @@ scan_fwd_kernel(ScanParams p) {
     for (int w = warp; w < SCAN_WARPS; ++w) whole.then(maps.get(buf, w, lane));
     Lanes<VEC> mine = carry;
     if (p.cluster > 1) {
-      put_in_cluster<VEC, PACKED>(blocks, buf, at.rank, p.cluster, warp, lane, whole);
-      cluster_arrive();
-      cluster_wait();
+      if (warp < p.cluster) blocks.send_to(warp, buf, at.rank, lane, whole);
+      if (threadIdx.x == 0) blocks.expect(buf, p.cluster);
+      blocks.wait(buf, round >> 1, ring.wait_ctl);
       for (int k = 0; k < p.cluster; ++k) {
         if (k == at.rank) mine = carry;
         blocks.get(buf, k, lane).apply(carry);
@@ -388,14 +514,20 @@ scan_fwd_kernel(ScanParams p) {
   }
   // Rows past T are identity maps (a = 1, x = 0), so the state behind the last tile is the one after the last token.
   if (!PACKED && p.final_state && warp == 0 && at.rank == 0 && active) store_f32<VEC>(p.final_state + at.state, carry);
+  if (asks && ring.given_up()) ring.drain();
+  if (p.cluster > 1) cluster_barrier();          // a block stays while others may send to it
 }
 
-template <typename TX, typename TG, int VEC, bool PACKED>
-__global__ void __launch_bounds__(32 * SCAN_WARPS)
-scan_bwd_kernel(ScanParams p) {
+template <typename TX, typename TG, bool RING, bool PACKED>
+__global__ void __launch_bounds__(32 * SCAN_WARPS, sizeof(TX) + sizeof(TG) == 4 ? 2 : 1)
+scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
+  constexpr int VEC = RING ? 2 : 1;
   using MapT = Map<VEC, PACKED>;
+  using BlockMaps = ClusterMaps<VEC, PACKED>;
+  extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ SharedMaps<VEC, SCAN_WARPS, PACKED> maps, reverse_maps;
-  __shared__ SharedMaps<VEC, SCAN_MAX_CLUSTER, PACKED> blocks;
+  __shared__ RingControl control;
+  BlockMaps& blocks = *reinterpret_cast<BlockMaps*>(dynamic + (RING ? p.stages * Ring<TX, TG, true>::BYTES : 0));
   const Place<VEC> at(p);
   const int lane = at.lane, warp = at.warp, c0 = at.c0;
   const bool active = at.active;
@@ -403,7 +535,13 @@ scan_bwd_kernel(ScanParams p) {
   // mu behind the round's tiles, the same in every warp of the cluster
   Lanes<VEC> carry = load_f32<VEC>(p.dfinal + at.state, !PACKED && p.dfinal && active);
 
-  const int rounds = (p.tiles + p.cluster - 1) / p.cluster;
+  const int step = p.cluster * SCAN_TILE, rounds = (p.tiles + p.cluster - 1) / p.cluster, last = (rounds - 1) * step + at.rank * SCAN_TILE;
+  Ring<TX, TG, true> ring(tensors, dynamic, &control, p.status, at.slice0, at.b, RING ? p.stages : 0);
+  const bool asks = RING && threadIdx.x == 0;
+  if (p.cluster > 1) {
+    if (threadIdx.x == 0) blocks.init();
+    cluster_barrier();
+  }
   RawRows<TX, VEC> xr, hr;
   RawRows<TG, VEC> gr;
   auto request = [&](int t0) {
@@ -411,18 +549,35 @@ scan_bwd_kernel(ScanParams p) {
     request_rows<TG, VEC>(p.g, gb, t0, p.T, gr);
     request_rows<TX, VEC>(p.dh, hb, t0, p.T, hr);
   };
-  request(((rounds - 1) * p.cluster + at.rank) * SCAN_TILE + warp * SCAN_ROWS);
-  for (int round = rounds - 1; round >= 0; --round) {
-    const int tile = round * p.cluster + at.rank, t0 = tile * SCAN_TILE + warp * SCAN_ROWS, buf = round & 1;
+  auto saved = [&](int tile) {                   // the state before a tile
+    return load_f32<VEC>(p.carry + (static_cast<int64_t>(at.b) * p.tiles + tile) * p.D + c0, active && tile >= 0 && tile < p.tiles);
+  };
+  if (asks)
+    for (int n = 0; n < p.stages && n < rounds; ++n) ring.request(last - n * step);
+  if (!RING) request(last + warp * SCAN_ROWS);
+  int code = row_code<PACKED>(p, last + warp * SCAN_ROWS, lane);
+  Lanes<VEC> next_h = saved((rounds - 1) * p.cluster + at.rank);
+  for (int turn = 0; turn < rounds; ++turn) {
+    const int round = rounds - 1 - turn, tile = round * p.cluster + at.rank, t0 = tile * SCAN_TILE + warp * SCAN_ROWS, buf = turn & 1;
     Lanes<VEC> a[SCAN_ROWS], x[SCAN_ROWS], dh[SCAN_ROWS];
+    if (RING) {
+      const uint8_t* here = ring.wait();
+      take_rows<TX, VEC>(here, warp, lane, xr);
+      take_rows<TG, VEC>(here + ring.X_BYTES, warp, lane, gr);
+      take_rows<TX, VEC>(here + ring.X_BYTES + ring.G_BYTES, warp, lane, hr);
+      ring.advance();
+    }
     unpack_rows<TX, VEC>(xr, x);
     unpack_rows<TG, VEC>(gr, a);
     unpack_rows<TX, VEC>(hr, dh);
-    if (round > 0) request(t0 - p.cluster * SCAN_TILE);
-    const RowDocs docs = row_docs<PACKED>(p, t0, lane);
+    if (!RING && round > 0) request(t0 - step);
+    const RowDocs docs = row_docs<PACKED>(p, t0, code);
     const bool cuts = PACKED && docs.any();
-    // the state before the tile
-    Lanes<VEC> h = load_f32<VEC>(p.carry + (static_cast<int64_t>(at.b) * p.tiles + tile) * p.D + c0, active && tile < p.tiles);
+    Lanes<VEC> h = next_h;
+    if (round > 0) {
+      code = row_code<PACKED>(p, t0 - step, lane);
+      next_h = saved(tile - p.cluster);
+    }
     decays<VEC>(a);
     MapT run = MapT::identity(), back = run;
     if (cuts) {
@@ -447,6 +602,7 @@ scan_bwd_kernel(ScanParams p) {
     maps.put(buf, warp, lane, run);
     reverse_maps.put(buf, warp, lane, back);
     __syncthreads();
+    if (asks && round - p.stages >= 0 && !ring.given_up()) ring.request(last - (turn + p.stages) * step);
 
     MapT whole = MapT::identity();
 #pragma unroll 2
@@ -455,8 +611,8 @@ scan_bwd_kernel(ScanParams p) {
 #pragma unroll 2
     for (int w = warp; w >= 0; --w) whole.then(reverse_maps.get(buf, w, lane));
     if (p.cluster > 1) {
-      put_in_cluster<VEC, PACKED>(blocks, buf, at.rank, p.cluster, warp, lane, whole);
-      cluster_arrive();
+      if (warp < p.cluster) blocks.send_to(warp, buf, at.rank, lane, whole);
+      if (threadIdx.x == 0) blocks.expect(buf, p.cluster);
     }
     MapT before = MapT::identity();
 #pragma unroll 2
@@ -481,7 +637,7 @@ scan_bwd_kernel(ScanParams p) {
     }
     Lanes<VEC> mu = carry;
     if (p.cluster > 1) {
-      cluster_wait();
+      blocks.wait(buf, turn >> 1, ring.wait_ctl);
       for (int k = p.cluster - 1; k >= 0; --k) {
         if (k == at.rank) mu = carry;
         blocks.get(buf, k, lane).apply(carry);
@@ -512,6 +668,8 @@ scan_bwd_kernel(ScanParams p) {
     }
   }
   if (!PACKED && p.dinitial && warp == 0 && at.rank == 0 && active) store_f32<VEC>(p.dinitial + at.state, carry);
+  if (asks && ring.given_up()) ring.drain();
+  if (p.cluster > 1) cluster_barrier();          // a block stays while others may send to it
 }
 
 // One token: state <- exp(g) state + x in place, h the new state in x's type.  A stream over the state.
@@ -561,46 +719,85 @@ using namespace tgdn;
 
 namespace {
 
-template <bool BACKWARD, typename TX, typename TG, int VEC, bool PACKED>
+#define TRY_MAP(expr) do { if (const int rc_ = (expr)) return rc_; } while (0)
+
+// A (B, T, D) tensor for the copy engine, tiles of 64 channels of 128 tokens; rows past T and channels past D arrive as zeros.
+template <typename T>
+int scan_map_of(CUtensorMap* map, const ScanIn& in, int B, int T_, int D) {
+  const int64_t row = in.st ? in.st : D;         // an axis of size one has no stride to speak of: any valid one will do
+  return tgdn_make_typed_rows_map(map, in.p, sizeof(T) == 4 ? TGDN_F32 : std::is_same<T, __half>::value ? TGDN_F16 : TGDN_BF16, D, T_, B, row,
+                                  B > 1 ? in.sb : row * T_, 64, SCAN_TILE);
+}
+
+template <bool BACKWARD, typename TX, typename TG, bool RING, bool PACKED>
 int launch_scan(ScanParams p, cudaStream_t s) {
+  constexpr int VEC = RING ? 2 : 1;
   p.slices = (p.D + 32 * VEC - 1) / (32 * VEC);
   const int64_t units = static_cast<int64_t>(p.B) * p.slices;
+  const int sms = tgdn_sm_count();
   p.cluster = 1;
-  while (p.cluster < SCAN_MAX_CLUSTER && p.cluster < p.tiles && units * p.cluster * 2 <= tgdn_sm_count()) p.cluster *= 2;
+  while (p.cluster < SCAN_MAX_CLUSTER && p.cluster < p.tiles && units * p.cluster * 2 <= sms) p.cluster *= 2;
   if (units * p.cluster > 0x7fffffffLL) return TGDN_ERR_SHAPE;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(units * p.cluster));
-  config.blockDim = dim3(32 * SCAN_WARPS);
-  config.stream = s;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = static_cast<unsigned>(p.cluster);
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  config.attrs = &attribute;
-  config.numAttrs = p.cluster > 1 ? 1 : 0;
-  if constexpr (BACKWARD) return tgdn_cuda_error(cudaLaunchKernelEx(&config, scan_bwd_kernel<TX, TG, VEC, PACKED>, p));
-  else return tgdn_cuda_error(cudaLaunchKernelEx(&config, scan_fwd_kernel<TX, TG, VEC, PACKED>, p));
+  constexpr int fixed = (BACKWARD ? 2 : 1) * static_cast<int>(sizeof(SharedMaps<VEC, SCAN_WARPS, PACKED>)) + 256;   // static shared memory, and some
+  ScanMaps maps{};
+  int bytes = p.cluster > 1 ? static_cast<int>(sizeof(ClusterMaps<VEC, PACKED>)) : 0;
+  if constexpr (RING) {
+    TRY_MAP(scan_map_of<TX>(&maps.x, p.x, p.B, p.T, p.D));
+    TRY_MAP(scan_map_of<TG>(&maps.g, p.g, p.B, p.T, p.D));
+    if (BACKWARD) TRY_MAP(scan_map_of<TX>(&maps.dh, p.dh, p.B, p.T, p.D));
+    constexpr int stage = Ring<TX, TG, BACKWARD>::BYTES;
+    const int two = (228 * 1024 / 2 - 1024 - fixed - bytes) / stage, one = (227 * 1024 - fixed - bytes) / stage;
+    // Two blocks an SM wherever two stages leave room: with more blocks than SMs, and in clusters, whose eight blocks must find SMs of one
+    // part of the chip free at the same time (packed, 131072 x 1024, 16 clusters: 457 us forward with two stages, 700 with four).
+    p.stages = (units * p.cluster > sms || p.cluster > 1) && two >= 2 ? two : one;
+    if (p.stages > SCAN_MAX_STAGES) p.stages = SCAN_MAX_STAGES;
+    bytes += p.stages * stage;
+  }
+  auto launch = [&](auto kernel) -> int {
+    static bool configured[64] = {false};
+    if (const int rc = tgdn_dynamic_smem(reinterpret_cast<const void*>(kernel), 227 * 1024 - fixed, configured)) return rc;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(units * p.cluster));
+    config.blockDim = dim3(32 * SCAN_WARPS);
+    config.dynamicSmemBytes = bytes;
+    config.stream = s;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = static_cast<unsigned>(p.cluster);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = p.cluster > 1 ? 1 : 0;
+    return tgdn_cuda_error(cudaLaunchKernelEx(&config, kernel, maps, p));
+  };
+  if constexpr (BACKWARD) return launch(scan_bwd_kernel<TX, TG, RING, PACKED>);
+  else return launch(scan_fwd_kernel<TX, TG, RING, PACKED>);
 }
 
 template <bool BACKWARD, typename TX, typename TG>
-int launch_scan_of(const ScanParams& p, bool pairs, cudaStream_t s) {
-  if (pairs) return p.map ? launch_scan<BACKWARD, TX, TG, 2, true>(p, s) : launch_scan<BACKWARD, TX, TG, 2, false>(p, s);
-  return p.map ? launch_scan<BACKWARD, TX, TG, 1, true>(p, s) : launch_scan<BACKWARD, TX, TG, 1, false>(p, s);
+int launch_scan_of(const ScanParams& p, bool pieces, cudaStream_t s) {
+  if (pieces) return p.map ? launch_scan<BACKWARD, TX, TG, true, true>(p, s) : launch_scan<BACKWARD, TX, TG, true, false>(p, s);
+  return p.map ? launch_scan<BACKWARD, TX, TG, false, true>(p, s) : launch_scan<BACKWARD, TX, TG, false, false>(p, s);
 }
 
 template <bool BACKWARD>
-int launch_scan_any(const ScanParams& p, int xt, int gt, bool pairs, cudaStream_t s) {
-  if (xt == TGDN_F32 && gt == TGDN_F32) return launch_scan_of<BACKWARD, float, float>(p, pairs, s);
-  if (xt == TGDN_BF16 && gt == TGDN_F32) return launch_scan_of<BACKWARD, __nv_bfloat16, float>(p, pairs, s);
-  if (xt == TGDN_BF16 && gt == TGDN_BF16) return launch_scan_of<BACKWARD, __nv_bfloat16, __nv_bfloat16>(p, pairs, s);
-  if (xt == TGDN_F16 && gt == TGDN_F32) return launch_scan_of<BACKWARD, __half, float>(p, pairs, s);
-  if (xt == TGDN_F16 && gt == TGDN_F16) return launch_scan_of<BACKWARD, __half, __half>(p, pairs, s);
+int launch_scan_any(const ScanParams& p, int xt, int gt, bool pieces, cudaStream_t s) {
+  if (xt == TGDN_F32 && gt == TGDN_F32) return launch_scan_of<BACKWARD, float, float>(p, pieces, s);
+  if (xt == TGDN_BF16 && gt == TGDN_F32) return launch_scan_of<BACKWARD, __nv_bfloat16, float>(p, pieces, s);
+  if (xt == TGDN_BF16 && gt == TGDN_BF16) return launch_scan_of<BACKWARD, __nv_bfloat16, __nv_bfloat16>(p, pieces, s);
+  if (xt == TGDN_F16 && gt == TGDN_F32) return launch_scan_of<BACKWARD, __half, float>(p, pieces, s);
+  if (xt == TGDN_F16 && gt == TGDN_F16) return launch_scan_of<BACKWARD, __half, __half>(p, pieces, s);
   return TGDN_ERR_TYPE;
 }
 
-ScanIn scan_in(const tgdn_rows& t) { return {t.data, t.stride_outer, static_cast<int>(t.stride_inner)}; }
+ScanIn scan_in(const tgdn_rows& t, int T) { return {t.data, t.stride_outer, T == 1 ? 0 : static_cast<int>(t.stride_inner)}; }
 
-bool in_pairs(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % (2 * type_bytes(type)) == 0; }
+// What the copy engine takes: rows of whole 16-byte pieces, axes that advance.  Pairs of the outputs follow from D.
+bool in_pieces(const tgdn_rows& t, int B, int T, int D) {
+  const int64_t piece = 16 / type_bytes(t.type);
+  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && D % piece == 0 && (T == 1 || (t.stride_inner > 0 && t.stride_inner % piece == 0)) &&
+         (B == 1 || (t.stride_outer > 0 && t.stride_outer % piece == 0 && t.stride_outer < int64_t{1} << 36));
+}
+bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 int scan_checks(const tgdn_rows* x, const tgdn_rows* g, const int32_t* map, int n_docs, int B, int T, int D) {
   if (!x || !g || !x->data || !g->data) return TGDN_ERR_NULL;
@@ -630,13 +827,14 @@ extern "C" int tgdn_scan_fwd(const tgdn_rows* host_x, const tgdn_rows* host_g, c
   if (!h) return TGDN_ERR_NULL;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   ScanParams p{};
-  p.x = scan_in(*host_x);
-  p.g = scan_in(*host_g);
+  p.x = scan_in(*host_x, T);
+  p.g = scan_in(*host_g, T);
   p.map = map; p.initial = initial; p.h = h; p.final_state = final_state; p.carry = carry;
   p.B = B; p.T = T; p.D = D; p.n_docs = n_docs;
   p.tiles = (T - 1) / SCAN_TILE + 1;
-  const bool pairs = D % 2 == 0 && rows_in_vectors(*host_x, 2) && rows_in_vectors(*host_g, 2) && in_pairs(h, host_x->type);
-  return launch_scan_any<false>(p, host_x->type, host_g->type, pairs, static_cast<cudaStream_t>(stream));
+  const bool pieces = in_pieces(*host_x, B, T, D) && in_pieces(*host_g, B, T, D) && aligned(h, 8);
+  p.status = tgdn_status_word();
+  return launch_scan_any<false>(p, host_x->type, host_g->type, pieces, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tgdn_scan_bwd(const tgdn_rows* host_x, const tgdn_rows* host_g, const tgdn_rows* host_dh, const int32_t* map, int n_docs,
@@ -648,16 +846,16 @@ extern "C" int tgdn_scan_bwd(const tgdn_rows* host_x, const tgdn_rows* host_g, c
   if (host_dh->stride_inner > 0x7fffffffLL || host_dh->stride_inner < 0) return TGDN_ERR_SHAPE;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   ScanParams p{};
-  p.x = scan_in(*host_x);
-  p.g = scan_in(*host_g);
-  p.dh = scan_in(*host_dh);
+  p.x = scan_in(*host_x, T);
+  p.g = scan_in(*host_g, T);
+  p.dh = scan_in(*host_dh, T);
   p.map = map; p.initial = initial; p.carry = const_cast<float*>(carry); p.dfinal = dfinal;
   p.dx = dx; p.dg = dg; p.dinitial = dinitial;
   p.B = B; p.T = T; p.D = D; p.n_docs = n_docs;
   p.tiles = (T - 1) / SCAN_TILE + 1;
-  const bool pairs = D % 2 == 0 && rows_in_vectors(*host_x, 2) && rows_in_vectors(*host_g, 2) && rows_in_vectors(*host_dh, 2) &&
-                     in_pairs(dx, host_x->type) && in_pairs(dg, host_g->type);
-  return launch_scan_any<true>(p, host_x->type, host_g->type, pairs, static_cast<cudaStream_t>(stream));
+  const bool pieces = in_pieces(*host_x, B, T, D) && in_pieces(*host_g, B, T, D) && in_pieces(*host_dh, B, T, D) && aligned(dx, 8) && aligned(dg, 8);
+  p.status = tgdn_status_word();
+  return launch_scan_any<true>(p, host_x->type, host_g->type, pieces, static_cast<cudaStream_t>(stream));
 }
 
 namespace {
