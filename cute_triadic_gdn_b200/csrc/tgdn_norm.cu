@@ -3,89 +3,105 @@
 
 namespace tgdn {
 
-template <typename TX, typename TR, int VEC, int K, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_fwd_kernel(NormParams p) {
+template <typename TX, typename TR, int VEC, bool EDGES, int SIZE>
+__global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 3 : 1) residual_fwd_kernel(NormParams p) {
+  constexpr int E = NORM_CHANNELS, K = E / VEC;
+  extern __shared__ float4 vectors[];
   __shared__ float red[2][NORM_MAX_WARPS];
-  const int tpr = p.tpr, lane = threadIdx.x % tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
-  float w[K][VEC], c[K][VEC];
-  load_small<VEC, K>(p.weight, 1.f, lane, tpr, p.N, w);
-  load_small<VEC, K>(p.scale, p.scale_value, lane, tpr, p.N, c);
-  int phase = 0;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < p.rows; base += static_cast<int64_t>(gridDim.x) * groups) {
-    const int64_t row = base + group;
+  Walk<VEC, K, EDGES> walk(p);
+  RawRow<TX, VEC, K, EDGES> xr;
+  RawRow<TR, VEC, K, EDGES> rr;
+  auto request = [&](int64_t row) {              // the next row is on its way while this one is worked on
     const bool ok = row < p.rows;
-    float x[K][VEC], r[K][VEC];
-    const uint32_t rr = ok ? static_cast<uint32_t>(row) : 0u;
-    load_row<TX, VEC, K>(static_cast<const TX*>(p.x.p) + p.x.at(rr), ok, lane, tpr, p.N, x);
-    load_row<TR, VEC, K>(static_cast<const TR*>(p.other.p) + p.other.at(rr), ok, lane, tpr, p.N, r);
-    float ss = 0.f;
+    const bool last = row >= p.rows - p.end_rows;
+    const uint32_t r = ok ? static_cast<uint32_t>(row) : 0u;
+    xr.load(static_cast<const TX*>(p.x.p) + p.x.at(r), ok, last, walk.cols);
+    rr.load(static_cast<const TR*>(p.other.p) + p.other.at(r), ok, last, walk.cols);
+  };
+  request(walk.row());
+  Held<E> weight(vectors, 0), scale(vectors, 1);
+  weight.put(load_small<VEC, K, EDGES>(p.weight, 1.f, walk.cols));
+  scale.put(load_small<VEC, K, EDGES>(p.scale, p.scale_value, walk.cols));
+  for (int phase = 0; walk.base < p.rows; walk.base += walk.step, phase ^= 1) {
+    const int64_t row = walk.row();
+    const bool ok = row < p.rows;
+    const Row<E> x = xr.get(walk.cols);
+    Row<E> r = rr.get(walk.cols);
+    request(row + walk.step);
+    const Row<E> c = scale.get();
+    float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int i = 0; i < E; i += 2) {
+      r.set(i, __ffma2_rn(c.pair(i), x.pair(i), r.pair(i)));
+      ss = __ffma2_rn(r.pair(i), r.pair(i), ss);
+    }
+    store_row<TR, VEC, K, EDGES>(static_cast<TR*>(p.stream) + row * p.N, ok, walk.cols, r);
+    const float inv = rsqrtf(fmaf(row_sum(ss, walk.tpr, red, phase), p.inv_n, p.eps));
+    const Row<E> w = weight.get();
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        r[k][i] = fmaf(c[k][i], x[k][i], r[k][i]);
-        ss = fmaf(r[k][i], r[k][i], ss);
-      }
-    store_row<TR, VEC, K>(static_cast<TR*>(p.stream) + row * p.N, ok, lane, tpr, p.N, r);
-    const float inv = rsqrtf(fmaf(row_sum(ss, tpr, red, phase), p.inv_n, p.eps));
-    phase ^= 1;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) r[k][i] *= inv * w[k][i];
-    store_row<TX, VEC, K>(static_cast<TX*>(p.out) + row * p.N, ok, lane, tpr, p.N, r);
-    if (ok && lane == 0 && p.rstd) p.rstd[row] = inv;
+    for (int i = 0; i < E; i += 2) r.set(i, __fmul2_rn(__fmul2_rn(r.pair(i), make_float2(inv, inv)), w.pair(i)));
+    store_row<TX, VEC, K, EDGES>(static_cast<TX*>(p.out) + row * p.N, ok, walk.cols, r);
+    if (ok && walk.lane == 0 && p.rstd) p.rstd[row] = inv;
   }
 }
 
-template <typename TX, typename TR, int VEC, int K, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_bwd_kernel(NormParams p) {
+template <typename TX, typename TR, int VEC, bool EDGES, int SIZE>
+__global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 2 : 1) residual_bwd_kernel(NormParams p) {
+  constexpr int E = NORM_CHANNELS, K = E / VEC;
+  extern __shared__ float4 vectors[];
   __shared__ float red[2][NORM_MAX_WARPS];
-  __shared__ float area[NORM_BLOCK * VEC * K];
-  const int tpr = p.tpr, lane = threadIdx.x % tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
-  float w[K][VEC], c[K][VEC], dw[K][VEC], dc[K][VEC];
-  load_small<VEC, K>(p.weight, 1.f, lane, tpr, p.N, w);
-  load_small<VEC, K>(p.scale, p.scale_value, lane, tpr, p.N, c);
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) dw[k][i] = dc[k][i] = 0.f;
-  int phase = 0;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < p.rows; base += static_cast<int64_t>(gridDim.x) * groups) {
-    const int64_t row = base + group;
+  Walk<VEC, K, EDGES> walk(p);
+  RawRow<TR, VEC, K, EDGES> nr, sr;
+  RawRow<TX, VEC, K, EDGES> yr, xr;
+  constexpr bool AHEAD = SIZE == NORM_GROUPS;   // (one wide row a block: registers are short, and several blocks take turns)
+  float next_inv;
+  auto request = [&](int64_t row) {
     const bool ok = row < p.rows;
-    const uint32_t rr = ok ? static_cast<uint32_t>(row) : 0u;
-    float n[K][VEC], dy[K][VEC], ds[K][VEC], x[K][VEC];
-    load_row<TR, VEC, K>(static_cast<const TR*>(p.stream) + rr * static_cast<int64_t>(p.N), ok, lane, tpr, p.N, n);
-    load_row<TX, VEC, K>(static_cast<const TX*>(p.dy.p) + p.dy.at(rr), ok && p.dy.p, lane, tpr, p.N, dy);
-    load_row<TR, VEC, K>(static_cast<const TR*>(p.dstream.p) + p.dstream.at(rr), ok && p.dstream.p, lane, tpr, p.N, ds);
-    if (p.sums1) load_row<TX, VEC, K>(static_cast<const TX*>(p.x.p) + p.x.at(rr), ok, lane, tpr, p.N, x);
-    const float inv = ok ? p.rstd[row] : 0.f;
-    float s = 0.f;
+    const bool last = row >= p.rows - p.end_rows;
+    const uint32_t r = ok ? static_cast<uint32_t>(row) : 0u;
+    nr.load(static_cast<const TR*>(p.stream) + r * static_cast<int64_t>(p.N), ok, last, walk.cols);
+    yr.load(static_cast<const TX*>(p.dy.p) + p.dy.at(r), ok && p.dy.p, last, walk.cols);
+    sr.load(static_cast<const TR*>(p.dstream.p) + p.dstream.at(r), ok && p.dstream.p, last, walk.cols);
+    if (p.sums1) xr.load(static_cast<const TX*>(p.x.p) + p.x.at(r), ok, last, walk.cols);
+    next_inv = ok ? p.rstd[row] : 0.f;
+  };
+  if (AHEAD) request(walk.row());
+  Held<E> weight(vectors, 0), scale(vectors, 1);
+  weight.put(load_small<VEC, K, EDGES>(p.weight, 1.f, walk.cols));
+  scale.put(load_small<VEC, K, EDGES>(p.scale, p.scale_value, walk.cols));
+  Row<E> dw, dc;
+  dw.fill(0.f);
+  dc.fill(0.f);
+  for (int phase = 0; walk.base < p.rows; walk.base += walk.step, phase ^= 1) {
+    const int64_t row = walk.row();
+    const bool ok = row < p.rows;
+    if (!AHEAD) request(row);
+    Row<E> n = nr.get(walk.cols), dy = yr.get(walk.cols), ds = sr.get(walk.cols), x;
+    if (p.sums1) x = xr.get(walk.cols);
+    const float inv = next_inv;
+    if (AHEAD) request(row + walk.step);
+    const Row<E> w = weight.get();
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int i = 0; i < E; i += 2) {
+      n.set(i, __fmul2_rn(n.pair(i), make_float2(inv, inv)));
+      dw.set(i, __ffma2_rn(dy.pair(i), n.pair(i), dw.pair(i)));
+      dy.set(i, __fmul2_rn(dy.pair(i), w.pair(i)));
+      sum = __ffma2_rn(dy.pair(i), n.pair(i), sum);
+    }
+    const float s = -row_sum(sum, walk.tpr, red, phase) * p.inv_n;
+    const Row<E> c = scale.get();
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        n[k][i] *= inv;
-        dw[k][i] = fmaf(dy[k][i], n[k][i], dw[k][i]);
-        dy[k][i] *= w[k][i];
-        s = fmaf(dy[k][i], n[k][i], s);
-      }
-    s = row_sum(s, tpr, red, phase) * p.inv_n;
-    phase ^= 1;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        ds[k][i] = fmaf(inv, fmaf(-n[k][i], s, dy[k][i]), ds[k][i]);
-        if (p.sums1) dc[k][i] = fmaf(ds[k][i], x[k][i], dc[k][i]);
-        dy[k][i] = ds[k][i] * c[k][i];
-      }
-    store_row<TR, VEC, K>(static_cast<TR*>(p.dother) + row * p.N, ok, lane, tpr, p.N, ds);
-    if (p.dx) store_row<TX, VEC, K>(static_cast<TX*>(p.dx) + row * p.N, ok, lane, tpr, p.N, dy);
+    for (int i = 0; i < E; i += 2) {
+      ds.set(i, __ffma2_rn(make_float2(inv, inv), __ffma2_rn(n.pair(i), make_float2(s, s), dy.pair(i)), ds.pair(i)));
+      if (p.sums1) dc.set(i, __ffma2_rn(ds.pair(i), x.pair(i), dc.pair(i)));
+      dy.set(i, __fmul2_rn(ds.pair(i), c.pair(i)));
+    }
+    store_row<TR, VEC, K, EDGES>(static_cast<TR*>(p.dother) + row * p.N, ok, walk.cols, ds);
+    if (p.dx) store_row<TX, VEC, K, EDGES>(static_cast<TX*>(p.dx) + row * p.N, ok, walk.cols, dy);
   }
-  if (p.sums0) leave_sums<VEC, K>(dw, p.sums0, area, lane, group, groups, tpr, p.N);
-  if (p.sums1) leave_sums<VEC, K>(dc, p.sums1, area, lane, group, groups, tpr, p.N);
+  if (p.sums0) leave_sums<VEC, K, EDGES>(dw, p.sums0, reinterpret_cast<float*>(vectors), walk, p.N);
+  if (p.sums1) leave_sums<VEC, K, EDGES>(dc, p.sums1, reinterpret_cast<float*>(vectors), walk, p.N);
 }
 
 // Column sums of the partials, in the order of the blocks: thread (i, j) adds up every 32nd partial of channel j from the i-th on, then
@@ -152,9 +168,9 @@ extern "C" int tgdn_residual_norm_fwd(const tgdn_rows* host_x, const tgdn_rows* 
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   const int xt = host_x->type, rt = host_residual->type;
   const tgdn_rows yo = dense(y, xt, rows, N), so = dense(stream_out, rt, rows, N);
-  const NormShape s = norm_shape(N, vectors_ok(N, vec_of(xt), {host_x, host_residual, &yo, &so}), vec_of(xt));
+  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(xt), {host_x, host_residual, &yo, &so}), vec_of(xt));
   NormParams p = norm_params(rows, N, eps, s, host_weight, host_scale, scale_value);
-  p.x = rows_at(host_x); p.other = rows_at(host_residual); p.out = y; p.stream = stream_out; p.rstd = rstd;
+  p.x = rows_at(host_x, rows); p.other = rows_at(host_residual, rows); p.out = y; p.stream = stream_out; p.rstd = rstd;
   return launch_types<ResidualFwd>(xt, rt, s, norm_blocks(s, rows), p, static_cast<cudaStream_t>(stream));
 }
 
@@ -174,11 +190,11 @@ extern "C" int tgdn_residual_norm_bwd(const void* stream_in, int stream_type, co
   if ((host_dy && host_dy->data && host_dy->type != x_type) || (host_dstream && host_dstream->data && host_dstream->type != stream_type)) return TGDN_ERR_TYPE;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   const tgdn_rows si = dense(stream_in, stream_type, rows, N), dr = dense(dresidual, stream_type, rows, N), dxo = dense(dx, x_type, rows, N);
-  const NormShape s = norm_shape(N, vectors_ok(N, vec_of(x_type), {&si, &dr, &dxo, host_dy, host_dstream, want_c ? host_x : nullptr}), vec_of(x_type));
+  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(x_type), {&si, &dr, &dxo, host_dy, host_dstream, want_c ? host_x : nullptr}), vec_of(x_type));
   const int blocks = norm_blocks(s, rows);
   if ((want_w || want_c) && (!scratch || scratch_floats < 2 * static_cast<int64_t>(blocks) * N)) return TGDN_ERR_SCRATCH;
   NormParams p = norm_params(rows, N, 0.f, s, host_weight, host_scale, scale_value);
-  p.x = rows_at(want_c ? host_x : nullptr); p.dy = rows_at(host_dy); p.dstream = rows_at(host_dstream);
+  p.x = rows_at(want_c ? host_x : nullptr, rows); p.dy = rows_at(host_dy, rows); p.dstream = rows_at(host_dstream, rows);
   p.stream = const_cast<void*>(stream_in); p.rstd = const_cast<float*>(rstd); p.dother = dresidual; p.dx = dx;
   p.sums0 = want_w ? scratch : nullptr;
   p.sums1 = want_c ? scratch + static_cast<int64_t>(blocks) * N : nullptr;

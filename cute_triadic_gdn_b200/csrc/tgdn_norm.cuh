@@ -28,13 +28,17 @@ namespace tgdn {
 
 constexpr int NORM_BLOCK = 256;                  // threads of a block that holds several rows
 constexpr int NORM_MAX_WARPS = 32;
+constexpr int NORM_CHANNELS = 16;                 // of a row, a thread
+enum NormSize { NORM_GROUPS, NORM_WIDE, NORM_WIDEST };   // several rows a block; one row, up to 512 threads; up to 1024
+constexpr int norm_threads(int size) { return size == NORM_GROUPS ? NORM_BLOCK : size == NORM_WIDE ? 512 : 1024; }
 
 struct RowsAt {                                  // row r of the tensor starts at (r / inner) * so + (r % inner) * si
   const void* p;
   int64_t so, si;
-  uint32_t inner;
+  uint32_t inner, magic, shift;                  // inner = 0: one level, r * si;  r / inner = (mulhi(r, magic) + r) >> shift for r < 2^31
   __device__ __forceinline__ int64_t at(uint32_t r) const {
-    const uint32_t o = r / inner;
+    if (inner == 0) return r * si;
+    const uint32_t o = (__umulhi(r, magic) + r) >> shift;
     return o * so + (r - o * inner) * si;
   }
 };
@@ -56,11 +60,131 @@ struct NormParams {
   float scale_value, eps, inv_n;
   int64_t rows;
   int N, tpr, act;
+  int end_rows;                                  // so many rows at the end of a tensor have less than a vector behind them
+};
+
+// A thread's E channels of a row, worked on in pairs by the two-wide f32 instructions.
+template <int E>
+struct Row {
+  float v[E];
+  __device__ __forceinline__ float2 pair(int i) const { return make_float2(v[i], v[i + 1]); }
+  __device__ __forceinline__ void set(int i, float2 p) { v[i] = p.x, v[i + 1] = p.y; }
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = f;
+  }
+};
+
+// Which channels: its vectors of VEC, the k-th at ((k * tpr) + lane) * VEC - shift.  Rows of any length that follow one another densely start
+// `shift` elements behind a vector's border, the same shift for all rows of a group (the rows of a group are multiples of eight apart), so
+// that whole vectors are moved although N is no multiple of them; what sticks out at a row's two ends is left out, and written element by
+// element.
+template <int VEC, int K, bool EDGES>
+struct Columns {
+  int first, step, N;
+  __device__ __forceinline__ Columns(int lane, int tpr, int shift, int N_) : first(lane * VEC - shift), step(tpr * VEC), N(N_) {}
+  __device__ __forceinline__ int at(int k) const { return first + k * step; }
+  __device__ __forceinline__ bool whole(int c) const { return EDGES ? c >= 0 && c + VEC <= N : c < N; }
+  __device__ __forceinline__ bool part(int c) const { return EDGES && c + VEC > 0 && c < N; }
+  __device__ __forceinline__ bool holds(int c) const { return (!EDGES || c >= 0) && c < N; }
+};
+
+template <typename T, int VEC, int K, bool EDGES>
+struct RawRow {
+  Raw<T, VEC> raw[K];
+  // Vectors at a row's ends bring elements of its neighbours along, which get() leaves out; only the last rows, behind which the tensor
+  // ends, take their ends element by element (those reads are waited for at once).
+  __device__ __forceinline__ void load(const T* row, bool ok, bool last, const Columns<VEC, K, EDGES>& cols) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = cols.at(k);
+      raw[k].zero();
+      if (ok && (cols.whole(c) || (cols.part(c) && !last))) {
+        raw[k].load(row + c);
+      } else if (ok && cols.part(c)) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (cols.holds(c + i)) raw[k].load_one(row + c + i, i);
+      }
+    }
+  }
+  __device__ __forceinline__ Row<K * VEC> get(const Columns<VEC, K, EDGES>& cols) const {
+    Row<K * VEC> r;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      raw[k].get(r.v + k * VEC);
+      const int c = cols.at(k);
+      if (EDGES && !cols.whole(c)) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) r.v[k * VEC + i] = cols.holds(c + i) ? r.v[k * VEC + i] : 0.f;
+      }
+    }
+    return r;
+  }
+};
+template <typename T, int VEC, int K, bool EDGES>
+__device__ __forceinline__ void store_row(T* row, bool ok, const Columns<VEC, K, EDGES>& cols, const Row<K * VEC>& r) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = cols.at(k);
+    if (ok && cols.whole(c)) {
+      store_f32_as<T, VEC>(row + c, r.v + k * VEC);
+    } else if (ok && cols.part(c)) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (cols.holds(c + i)) row[c + i] = from_f32<T>(r.v[k * VEC + i]);
+    }
+  }
+}
+template <int VEC, int K, bool EDGES>
+__device__ __forceinline__ Row<K * VEC> load_small(const SmallVector& s, float otherwise, const Columns<VEC, K, EDGES>& cols) {
+  Row<K * VEC> r;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.v[k * VEC + i] = cols.holds(cols.at(k) + i) ? s.get(cols.at(k) + i, otherwise) : 0.f;
+  return r;
+}
+
+// A vector over the channels that every row needs, kept in shared memory: a slot per thread, which it alone writes and reads.
+template <int E>
+struct Held {
+  float4* slot;
+  int threads;
+  __device__ __forceinline__ Held(float4* area, int which) : slot(area + which * (E / 4) * blockDim.x + threadIdx.x), threads(blockDim.x) {}
+  __device__ __forceinline__ void put(const Row<E>& v) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) slot[i / 4 * threads] = make_float4(v.v[i], v.v[i + 1], v.v[i + 2], v.v[i + 3]);
+  }
+  __device__ __forceinline__ Row<E> get() const {
+    Row<E> v;
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const float4 q = slot[i / 4 * threads];
+      v.v[i] = q.x, v.v[i + 1] = q.y, v.v[i + 2] = q.z, v.v[i + 3] = q.w;
+    }
+    return v;
+  }
+};
+
+// The walk of a thread over its rows: group `group` of the block takes row base + group of every base, all groups together (they meet in
+// shuffles and barriers).
+template <int VEC, int K, bool EDGES>
+struct Walk {
+  int tpr, lane, group, groups;
+  int64_t base, step;
+  Columns<VEC, K, EDGES> cols;
+  __device__ __forceinline__ explicit Walk(const NormParams& p)
+      : tpr(p.tpr), lane(threadIdx.x % p.tpr), group(threadIdx.x / p.tpr), groups(blockDim.x / p.tpr),
+        base(static_cast<int64_t>(blockIdx.x) * groups), step(static_cast<int64_t>(gridDim.x) * groups),
+        cols(lane, p.tpr, EDGES ? static_cast<int>((base + group) * p.N % VEC) : 0, p.N) {}
+  __device__ __forceinline__ int64_t row() const { return base + group; }
 };
 
 // Sum over the `tpr` threads of a row; every one of them gets it.  Rows of several warps are one per block: `red` is double-buffered by
 // the caller (`phase`), so one barrier a sum is enough.
-__device__ __forceinline__ float row_sum(float v, int tpr, float (*red)[NORM_MAX_WARPS], int phase) {
+__device__ __forceinline__ float row_sum(float2 pair, int tpr, float (*red)[NORM_MAX_WARPS], int phase) {
+  float v = pair.x + pair.y;
   const int width = tpr < 32 ? tpr : 32;
   for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (tpr <= 32) return v;
@@ -71,58 +195,34 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float (*red)[NORM_MAX
   return s;
 }
 
-// A thread's channels of a row: K vectors of VEC, the k-th at ((k * tpr) + lane) * VEC.
-template <typename T, int VEC, int K>
-__device__ __forceinline__ void load_row(const T* row, bool ok, int lane, int tpr, int N, float (&out)[K][VEC]) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (k * tpr + lane) * VEC;
-    const Pack<T, VEC> raw = ok && c < N ? load_pack<T, VEC>(row + c) : zero_pack<T, VEC>();
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[k][i] = to_f32(raw.v[i]);
-  }
-}
-template <typename T, int VEC, int K>
-__device__ __forceinline__ void store_row(T* row, bool ok, int lane, int tpr, int N, const float (&v)[K][VEC]) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (k * tpr + lane) * VEC;
-    if (ok && c < N) store_pack<T, VEC>(row + c, v[k]);
-  }
-}
-template <int VEC, int K>
-__device__ __forceinline__ void load_small(const SmallVector& s, float otherwise, int lane, int tpr, int N, float (&out)[K][VEC]) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (k * tpr + lane) * VEC;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[k][i] = c < N ? s.get(c + i, otherwise) : 0.f;
-  }
-}
-
 // The sums that the threads of a block hold for the same channels, added up over its groups in their order, and left as the block's partial.
-template <int VEC, int K>
-__device__ __forceinline__ void leave_sums(const float (&v)[K][VEC], float* partial, float* area, int lane, int group, int groups, int tpr, int N) {
-  if (groups == 1) {
+template <int VEC, int K, bool EDGES>
+__device__ __forceinline__ void leave_sums(const Row<K * VEC>& s, float* partial, float* area, const Walk<VEC, K, EDGES>& walk, int N) {
+  float* out = partial + static_cast<int64_t>(blockIdx.x) * N;
+  if (walk.groups == 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const int c = (k * tpr + lane) * VEC + i;
-        if (c < N) partial[static_cast<int64_t>(blockIdx.x) * N + c] = v[k][i];
+        const int c = walk.cols.at(k) + i;
+        if (walk.cols.holds(c)) out[c] = s.v[k * VEC + i];
       }
     return;
   }
+  const int pitch = walk.tpr * K * VEC;          // at least N
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) area[group * (tpr * K * VEC) + (k * tpr + lane) * VEC + i] = v[k][i];
+    for (int i = 0; i < VEC; ++i) {
+      const int c = walk.cols.at(k) + i;
+      if (walk.cols.holds(c)) area[walk.group * pitch + c] = s.v[k * VEC + i];
+    }
   __syncthreads();
   for (int c = threadIdx.x; c < N; c += blockDim.x) {
-    float s = 0.f;
-    for (int g = 0; g < groups; ++g) s += area[g * (tpr * K * VEC) + c];
-    partial[static_cast<int64_t>(blockIdx.x) * N + c] = s;
+    float t = 0.f;
+    for (int g = 0; g < walk.groups; ++g) t += area[g * pitch + c];
+    out[c] = t;
   }
 }
 
@@ -135,17 +235,17 @@ int norm_add_up(const float* partials, int blocks, int N, const tgdn_vector* f0,
 namespace tgdn {
 namespace {
 
-// How a row is laid over threads: `tpr` threads of K vectors each.  Part of a warp (a power of two) as far as one vector a thread goes,
-// whole warps beyond; two vectors a thread above 128 threads, so that a block of a wide row has fewer warps to wait for.
+// How a row is laid over threads: `tpr` threads of sixteen channels each, a power of two of a warp's lanes as far as they go and whole warps
+// beyond.
 struct NormShape {
-  int vec, k, tpr, threads, groups;
+  int vec, tpr, threads, groups;
+  bool edges;
 };
 NormShape norm_shape(int N, bool vectors, int vec_elements) {
   NormShape s;
   s.vec = vectors ? vec_elements : 1;
-  const int per8 = 8 / s.vec, units = (N + s.vec - 1) / s.vec;         // vectors of eight channels' worth
-  s.k = (units + per8 - 1) / per8 > 128 ? 2 * per8 : per8;
-  const int need = (units + s.k - 1) / s.k;
+  s.edges = N % s.vec != 0;
+  const int units = (N + (s.edges ? s.vec - 1 : 0) + s.vec - 1) / s.vec, need = (units * s.vec + NORM_CHANNELS - 1) / NORM_CHANNELS;
   if (need <= 32) {
     s.tpr = 1;
     while (s.tpr < need) s.tpr *= 2;
@@ -154,28 +254,43 @@ NormShape norm_shape(int N, bool vectors, int vec_elements) {
     s.tpr = (need + 31) / 32 * 32;
     s.threads = s.tpr;
   }
+  if (s.threads > 1024) return norm_shape(N, false, vec_elements);     // (the widest rows, where they do not start on a vector's border)
   s.groups = s.threads / s.tpr;
   return s;
 }
 
-// Blocks of a pass: as many as hold the rows, at most two thousand threads' worth on every SM.
+// Blocks of a pass: as many as hold the rows, at most two thousand threads' worth on every SM; rows of a group are multiples of eight apart.
 int norm_blocks(const NormShape& s, int64_t rows) {
   const int64_t want = (rows + s.groups - 1) / s.groups, most = static_cast<int64_t>(tgdn_sm_count()) * (2048 / s.threads > 0 ? 2048 / s.threads : 1);
-  return static_cast<int>(want < most ? want : most);
+  const int multiple = s.groups >= 8 ? 1 : 8 / s.groups;
+  return static_cast<int>(((want < most ? want : most) + multiple - 1) / multiple * multiple);
 }
 
-bool vectors_ok(int N, int vec, std::initializer_list<const tgdn_rows*> tensors) {
-  if (N % vec) return false;
-  for (const tgdn_rows* t : tensors)
-    if (t && t->data && !rows_in_vectors(*t, vec)) return false;
+// True when the rows can be moved as vectors: every row starts as far behind a vector's border as row * N elements do, and what a vector
+// at a row's end takes along lies in the rows behind it.
+bool vectors_ok(int64_t rows, int N, int vec, std::initializer_list<const tgdn_rows*> tensors) {
+  for (const tgdn_rows* t : tensors) {
+    if (!t || !t->data) continue;
+    if (reinterpret_cast<uintptr_t>(t->data) % 16) return false;
+    if (t->stride_inner % vec != N % vec) return false;
+    if (N % vec && (t->stride_inner < N || (t->inner < rows && t->stride_outer < t->inner * t->stride_inner))) return false;
+    if (t->inner < rows && t->stride_outer % vec != static_cast<int64_t>(t->inner % vec) * (N % vec) % vec) return false;
+  }
   return true;
 }
 
-RowsAt rows_at(const tgdn_rows* t) {
-  if (!t || !t->data) return RowsAt{nullptr, 0, 0, 1u};
-  return RowsAt{t->data, t->stride_outer, t->stride_inner, static_cast<uint32_t>(t->inner)};
+RowsAt rows_at(const tgdn_rows* t, int64_t rows) {
+  RowsAt r{};
+  if (!t || !t->data) return r;
+  r.p = t->data; r.so = t->stride_outer; r.si = t->stride_inner;
+  if (r.so == r.si * t->inner || t->inner >= rows) return r;
+  r.inner = static_cast<uint32_t>(t->inner);
+  while ((uint64_t{1} << r.shift) < r.inner) ++r.shift;
+  r.magic = static_cast<uint32_t>(((uint64_t{1} << 32) * ((uint64_t{1} << r.shift) - r.inner)) / r.inner + 1);
+  return r;
 }
-tgdn_rows dense(const void* p, int type, int64_t rows, int N) { return tgdn_rows{p, rows > 0 ? rows : 1, 0, N, type}; }
+// (one level: rows of an outer stride that the kernels never read)
+tgdn_rows dense(const void* p, int type, int64_t rows, int N) { return tgdn_rows{p, rows, rows * N, N, type}; }
 SmallVector small(const tgdn_vector* v) { return v && v->data ? SmallVector{v->data, v->type} : SmallVector{nullptr, 0}; }
 
 int check_rows(const tgdn_rows* t, bool needed) {
@@ -187,23 +302,28 @@ int check_vector(const tgdn_vector* v) { return v && v->data && !type_known(v->t
 
 #define TGDN_TRY(expr) do { if (const int rc_ = (expr)) return rc_; } while (0)
 
-// The kernels by shape: 16-byte vectors (eight channels of 16 bits, four of 32) or single channels; eight channels a thread, or sixteen in
-// blocks of up to 512 and of up to 1024 threads (whose registers differ).
-template <typename TX, typename TR, template <typename, typename, int, int, int> class Launch>
+// The kernels by shape: 16-byte vectors (eight channels of 16 bits, four of 32), the same with rows that start inside one, or single
+// channels; several rows a block, one of up to 512 threads or one of up to 1024 (whose registers differ).
+template <typename TX, typename TR, int VEC, bool EDGES, template <typename, typename, int, bool, int> class Launch>
+int launch_size(const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {
+  if (s.tpr <= 32) return Launch<TX, TR, VEC, EDGES, NORM_GROUPS>::go(s, blocks, p, st);
+  return s.threads <= 512 ? Launch<TX, TR, VEC, EDGES, NORM_WIDE>::go(s, blocks, p, st) : Launch<TX, TR, VEC, EDGES, NORM_WIDEST>::go(s, blocks, p, st);
+}
+template <typename TX, typename TR, template <typename, typename, int, bool, int> class Launch>
 int launch_shape(const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {
   constexpr int V = sizeof(TX) == 2 ? 8 : 4;
-  if (s.vec == V) {
-    if (s.k == 8 / V) Launch<TX, TR, V, 8 / V, NORM_BLOCK>::go(s, blocks, p, st);
-    else if (s.threads <= 512) Launch<TX, TR, V, 16 / V, 512>::go(s, blocks, p, st);
-    else Launch<TX, TR, V, 16 / V, 1024>::go(s, blocks, p, st);
-  } else {
-    if (s.k == 8) Launch<TX, TR, 1, 8, NORM_BLOCK>::go(s, blocks, p, st);
-    else if (s.threads <= 512) Launch<TX, TR, 1, 16, 512>::go(s, blocks, p, st);
-    else Launch<TX, TR, 1, 16, 1024>::go(s, blocks, p, st);
-  }
+  if (s.vec == 1) return launch_size<TX, TR, 1, false, Launch>(s, blocks, p, st);
+  return s.edges ? launch_size<TX, TR, V, true, Launch>(s, blocks, p, st) : launch_size<TX, TR, V, false, Launch>(s, blocks, p, st);
+}
+// Dynamic shared memory: two vectors over the channels (which the sums over a block's groups use after them).
+template <typename Kernel>
+int launch_norm(Kernel kernel, bool* configured, const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {
+  const int bytes = 2 * NORM_CHANNELS * 4 * s.threads;
+  if (const int rc = tgdn_dynamic_smem(reinterpret_cast<const void*>(kernel), 2 * NORM_CHANNELS * 4 * 1024, configured)) return rc;
+  kernel<<<blocks, s.threads, bytes, st>>>(p);
   return tgdn_cuda_error(cudaGetLastError());
 }
-template <template <typename, typename, int, int, int> class Launch>
+template <template <typename, typename, int, bool, int> class Launch>
 int launch_types(int xt, int rt, const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {
   if (xt == TGDN_F32 && rt == TGDN_F32) return launch_shape<float, float, Launch>(s, blocks, p, st);
   if (xt == TGDN_BF16 && rt == TGDN_BF16) return launch_shape<__nv_bfloat16, __nv_bfloat16, Launch>(s, blocks, p, st);
@@ -214,9 +334,10 @@ int launch_types(int xt, int rt, const NormShape& s, int blocks, const NormParam
 }
 
 #define TGDN_LAUNCHER(name, kernel)                                                                    \
-  template <typename TX, typename TR, int VEC, int K, int MAXT> struct name {                          \
-    static void go(const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {             \
-      kernel<TX, TR, VEC, K, MAXT><<<blocks, s.threads, 0, st>>>(p);                                   \
+  template <typename TX, typename TR, int VEC, bool EDGES, int SIZE> struct name {                     \
+    static int go(const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {              \
+      static bool configured[64] = {false};                                                            \
+      return launch_norm(kernel<TX, TR, VEC, EDGES, SIZE>, configured, s, blocks, p, st);              \
     }                                                                                                  \
   }
 
@@ -225,7 +346,7 @@ int check_norm(int64_t rows, int N) { return rows <= 0 || rows > 0x7fffffffLL ||
 NormParams norm_params(int64_t rows, int N, float eps, const NormShape& s, const tgdn_vector* weight, const tgdn_vector* scale, float scale_value) {
   NormParams p{};
   p.weight = small(weight); p.scale = small(scale); p.scale_value = scale_value; p.eps = eps; p.inv_n = 1.f / static_cast<float>(N);
-  p.rows = rows; p.N = N; p.tpr = s.tpr;
+  p.rows = rows; p.N = N; p.tpr = s.tpr; p.end_rows = (s.vec - 1 + N - 1) / N;
   return p;
 }
 

@@ -154,15 +154,20 @@ __device__ __forceinline__ RowDocs row_docs(const ScanParams& p, int t0, int cod
 // A tile's rows as they lie in memory: what a warp has in flight while it works on the tile before.
 template <typename T, int VEC>
 struct RawRows {
-  typename RawOf<VEC * sizeof(T)>::type v[SCAN_ROWS];
+  Raw<T, VEC> v[SCAN_ROWS];
 };
 
 // Reads that nothing else in the kernel writes, in the order they stand in (volatile: they must be under way before the work that hides
 // them), and past L1: no line is read twice by a block.
-__device__ __forceinline__ void read_once(uint16_t& d, const void* p) { asm volatile("ld.global.nc.L1::no_allocate.b16 %0, [%1];" : "=h"(d) : "l"(p)); }
-__device__ __forceinline__ void read_once(uint32_t& d, const void* p) { asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(d) : "l"(p)); }
-__device__ __forceinline__ void read_once(uint2& d, const void* p) {
-  asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(d.x), "=r"(d.y) : "l"(p));
+template <typename T>
+__device__ __forceinline__ void read_once(Raw<T, 1>& d, const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(d.w[0]) : "l"(p));
+  } else {
+    uint16_t v;
+    asm volatile("ld.global.nc.L1::no_allocate.b16 %0, [%1];" : "=h"(v) : "l"(p));
+    d.w[0] = v;
+  }
 }
 
 // Row r of a tile, for a stride below 2^31 elements (the launch checks): one wide product an address.  `stride` is made opaque once a tile, or
@@ -175,8 +180,8 @@ __device__ __forceinline__ int opaque(int v) {
 }
 
 // Rows past T read as zeros.  Lanes past D read channel 0 (`base` says so) and store nothing.
-template <typename T, int VEC>
-__device__ __forceinline__ void request_rows(const ScanIn& in, int64_t base, int t0, int T_, RawRows<T, VEC>& raw) {
+template <typename T>
+__device__ __forceinline__ void request_rows(const ScanIn& in, int64_t base, int t0, int T_, RawRows<T, 1>& raw) {
   const T* p = static_cast<const T*>(in.p) + base + static_cast<int64_t>(t0) * in.st;
   const int rows = T_ - t0, stride = opaque(in.st);
   if (rows >= SCAN_ROWS) {
@@ -185,7 +190,7 @@ __device__ __forceinline__ void request_rows(const ScanIn& in, int64_t base, int
   } else {
 #pragma unroll
     for (int r = 0; r < SCAN_ROWS; ++r) {
-      raw.v[r] = {};
+      raw.v[r].zero();
       if (r < rows) read_once(raw.v[r], row_of(p, r, stride));
     }
   }
@@ -193,12 +198,7 @@ __device__ __forceinline__ void request_rows(const ScanIn& in, int64_t base, int
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack_rows(const RawRows<T, VEC>& raw, Lanes<VEC> (&out)[SCAN_ROWS]) {
 #pragma unroll
-  for (int r = 0; r < SCAN_ROWS; ++r) {
-    union { typename RawOf<VEC * sizeof(T)>::type raw; Pack<T, VEC> pack; } u;
-    u.raw = raw.v[r];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[r].v[i] = to_f32(u.pack.v[i]);
-  }
+  for (int r = 0; r < SCAN_ROWS; ++r) raw.v[r].get(out[r].v);
 }
 
 // A map of a run of rows in a lane's channels: c -> A c + H, or c -> H where a document's border lies in the run (`cut`, one value for all
@@ -351,10 +351,9 @@ struct Ring {
 // A warp's rows of a tile in the ring, as they lie there.
 template <typename T, int VEC>
 __device__ __forceinline__ void take_rows(const uint8_t* tile, int warp, int lane, RawRows<T, VEC>& raw) {
-  using Raw = typename RawOf<VEC * sizeof(T)>::type;
-  const Raw* p = reinterpret_cast<const Raw*>(tile) + warp * SCAN_ROWS * 32 + lane;
+  const T* p = reinterpret_cast<const T*>(tile) + (warp * SCAN_ROWS * 32 + lane) * VEC;
 #pragma unroll
-  for (int r = 0; r < SCAN_ROWS; ++r) raw.v[r] = p[r * 32];
+  for (int r = 0; r < SCAN_ROWS; ++r) raw.v[r].load(p + r * 32 * VEC);
 }
 
 // Where a block stands: its slice of channels, its batch row, its place in the cluster.
@@ -434,9 +433,9 @@ scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   RawRows<TG, VEC> gr;
   if (asks)
     for (int n = 0; n < p.stages && n < rounds; ++n) ring.request(first + n * step);
-  if (!RING) {
-    request_rows<TX, VEC>(p.x, xb, first + warp * SCAN_ROWS, p.T, xr);
-    request_rows<TG, VEC>(p.g, gb, first + warp * SCAN_ROWS, p.T, gr);
+  if constexpr (!RING) {
+    request_rows<TX>(p.x, xb, first + warp * SCAN_ROWS, p.T, xr);
+    request_rows<TG>(p.g, gb, first + warp * SCAN_ROWS, p.T, gr);
   }
   int code = row_code<PACKED>(p, first + warp * SCAN_ROWS, lane);
   for (int round = 0; round < rounds; ++round) {
@@ -450,10 +449,11 @@ scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
     }
     unpack_rows<TX, VEC>(xr, x);
     unpack_rows<TG, VEC>(gr, a);
-    if (!RING && round + 1 < rounds) {
-      request_rows<TX, VEC>(p.x, xb, t0 + step, p.T, xr);
-      request_rows<TG, VEC>(p.g, gb, t0 + step, p.T, gr);
-    }
+    if constexpr (!RING)
+      if (round + 1 < rounds) {
+        request_rows<TX>(p.x, xb, t0 + step, p.T, xr);
+        request_rows<TG>(p.g, gb, t0 + step, p.T, gr);
+      }
     const RowDocs docs = row_docs<PACKED>(p, t0, code);
     if (round + 1 < rounds) code = row_code<PACKED>(p, t0 + step, lane);
     const bool cuts = PACKED && docs.any();
@@ -498,7 +498,7 @@ scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
 #pragma unroll
       for (int r = 0; r < SCAN_ROWS; ++r) {
         mine = docs.starts_at(r) ? x[r] : fma(a[r], mine, x[r]);
-        if (r < rows) store_pack<TX, VEC>(row_of(out, r, stride), mine.v);
+        if (r < rows) store_f32_as<TX, VEC>(row_of(out, r, stride), mine.v);
         if (p.final_state && docs.ends_at(r)) {
           const int doc = docs.closed(r);
           if (active && doc >= 0) store_f32<VEC>(p.final_state + static_cast<int64_t>(doc) * p.D + c0, mine);
@@ -508,7 +508,7 @@ scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
 #pragma unroll
       for (int r = 0; r < SCAN_ROWS; ++r) {
         mine = fma(a[r], mine, x[r]);
-        if (r < rows) store_pack<TX, VEC>(row_of(out, r, stride), mine.v);
+        if (r < rows) store_f32_as<TX, VEC>(row_of(out, r, stride), mine.v);
       }
     }
   }
@@ -545,9 +545,11 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   RawRows<TX, VEC> xr, hr;
   RawRows<TG, VEC> gr;
   auto request = [&](int t0) {
-    request_rows<TX, VEC>(p.x, xb, t0, p.T, xr);
-    request_rows<TG, VEC>(p.g, gb, t0, p.T, gr);
-    request_rows<TX, VEC>(p.dh, hb, t0, p.T, hr);
+    if constexpr (!RING) {
+      request_rows<TX>(p.x, xb, t0, p.T, xr);
+      request_rows<TG>(p.g, gb, t0, p.T, gr);
+      request_rows<TX>(p.dh, hb, t0, p.T, hr);
+    }
   };
   auto saved = [&](int tile) {                   // the state before a tile
     return load_f32<VEC>(p.carry + (static_cast<int64_t>(at.b) * p.tiles + tile) * p.D + c0, active && tile >= 0 && tile < p.tiles);
@@ -658,8 +660,8 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
       mu = mul(a[r], lam);
       const Lanes<VEC> d = mul(mu, x[r]);
       if (r < rows) {
-        store_pack<TX, VEC>(row_of(dx, r, stride), lam.v);
-        store_pack<TG, VEC>(row_of(dg, r, stride), d.v);
+        store_f32_as<TX, VEC>(row_of(dx, r, stride), lam.v);
+        store_f32_as<TG, VEC>(row_of(dg, r, stride), d.v);
       }
       if (cuts && p.dinitial && docs.starts_at(r)) {
         const int doc = docs.opened(r);
@@ -681,14 +683,20 @@ scan_step_kernel(const TX* x, int64_t x_row, const TG* g, int64_t g_row, float* 
   if (i >= vectors) return;
   const int64_t b = i / (D / VEC);
   const int c = static_cast<int>(i - b * (D / VEC)) * VEC;
-  const Pack<TX, VEC> xv = load_pack<TX, VEC>(x + b * x_row + c);
-  const Pack<TG, VEC> gv = load_pack<TG, VEC>(g + b * g_row + c);
-  const Pack<float, VEC> s = load_pack<float, VEC>(state + b * D + c);
-  float v[VEC];
+  Raw<TX, VEC> xr;
+  Raw<TG, VEC> gr;
+  Raw<float, VEC> sr;
+  xr.load(x + b * x_row + c);
+  gr.load(g + b * g_row + c);
+  sr.load(state + b * D + c);
+  float xv[VEC], gv[VEC], v[VEC];
+  xr.get(xv);
+  gr.get(gv);
+  sr.get(v);
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) v[k] = fmaf(decay<1>(Lanes<1>{{to_f32(gv.v[k])}}).v[0], s.v[k], to_f32(xv.v[k]));
-  store_pack<float, VEC>(state + b * D + c, v);
-  store_pack<TX, VEC>(h + b * D + c, v);
+  for (int k = 0; k < VEC; ++k) v[k] = fmaf(decay<1>(Lanes<1>{{gv[k]}}).v[0], v[k], xv[k]);
+  store_f32_as<float, VEC>(state + b * D + c, v);
+  store_f32_as<TX, VEC>(h + b * D + c, v);
 }
 
 // map[t] = d + 1 where document d opens at token t, else 0; valid = the offsets start at 0, end at T and strictly increase.  Offsets that
