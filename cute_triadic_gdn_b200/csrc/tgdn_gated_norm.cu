@@ -31,8 +31,8 @@ __device__ __forceinline__ float2 gate_act(bool silu, float2 z, float2& slope) {
 }
 
 template <typename TX, typename TR, int VEC, bool EDGES, int SIZE>
-__global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 3 : 1) gated_fwd_kernel(NormParams p) {
-  constexpr int E = NORM_CHANNELS, K = E / VEC;
+__global__ void TGDN_NORM_BOUNDS(false) gated_fwd_kernel(NormParams p) {
+  constexpr int E = norm_channels(sizeof(TX), SIZE), K = E / VEC;
   extern __shared__ float4 vectors[];
   __shared__ float red[2][NORM_MAX_WARPS];
   Walk<VEC, K, EDGES> walk(p);
@@ -65,6 +65,11 @@ __global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 3 : 
     const bool ok = row < p.rows;
     Row<E> x = xr.get(walk.cols);
     request(row + walk.step, true);
+    if (SIZE != NORM_GROUPS && threadIdx.x == 0 && row + walk.step < p.rows) {
+      const uint32_t r = static_cast<uint32_t>(row + walk.step);
+      if (p.act) pull_row(static_cast<const TX*>(p.other.p) + p.other.at(r), p.N);
+      if (p.residual.p) pull_row(static_cast<const TR*>(p.residual.p) + p.residual.at(r), p.N);
+    }
     float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < E; i += 2) ss = __ffma2_rn(x.pair(i), x.pair(i), ss);
@@ -92,8 +97,8 @@ __global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 3 : 
 }
 
 template <typename TX, typename TR, int VEC, bool EDGES, int SIZE>
-__global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 2 : 1) gated_bwd_kernel(NormParams p) {
-  constexpr int E = NORM_CHANNELS, K = E / VEC;
+__global__ void TGDN_NORM_BOUNDS(true) gated_bwd_kernel(NormParams p) {
+  constexpr int E = norm_channels(sizeof(TX), SIZE), K = E / VEC;
   extern __shared__ float4 vectors[];
   __shared__ float red[2][NORM_MAX_WARPS];
   Walk<VEC, K, EDGES> walk(p);
@@ -125,7 +130,15 @@ __global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 2 : 
   for (int phase = 0; walk.base < p.rows; walk.base += walk.step, phase ^= 1) {
     const int64_t row = walk.row();
     const bool ok = row < p.rows;
-    if (!AHEAD) request(row);
+    if (!AHEAD) {
+      request(row);
+      if (threadIdx.x == 0 && row + walk.step < p.rows) {
+        const uint32_t r = static_cast<uint32_t>(row + walk.step);
+        pull_row(static_cast<const TX*>(p.x.p) + p.x.at(r), p.N);
+        if (p.act) pull_row(static_cast<const TX*>(p.other.p) + p.other.at(r), p.N);
+        pull_row(static_cast<const TR*>(p.dy.p) + p.dy.at(r), p.N);
+      }
+    }
     Row<E> n = xr.get(walk.cols), z, dy = yr.get(walk.cols);
     if (p.act) z = zr.get(walk.cols);
     const float inv = next_inv;
@@ -175,10 +188,10 @@ extern "C" int tgdn_gated_norm_fwd(const tgdn_rows* host_x, const tgdn_rows* hos
   if (!type_known(out_type) || (gated && host_gate->type != xt) || (host_residual && host_residual->data && host_residual->type != out_type)) return TGDN_ERR_TYPE;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   const tgdn_rows oo = dense(out, out_type, rows, N);
-  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(xt), {host_x, gated ? host_gate : nullptr, host_residual, &oo}), vec_of(xt));
+  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(xt), {host_x, gated ? host_gate : nullptr, host_residual, &oo}), xt, out_type);
   NormParams p = norm_params(rows, N, eps, s, host_weight, host_scale, scale_value);
   p.x = rows_at(host_x, rows); p.other = rows_at(gated ? host_gate : nullptr, rows); p.residual = rows_at(host_residual, rows); p.out = out; p.rstd = rstd; p.act = activation;
-  const int blocks = norm_blocks(s, rows);
+  const int blocks = norm_blocks(s, rows, false);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return launch_types<GatedFwd>(xt, out_type, s, blocks, p, st);
 }
@@ -197,8 +210,8 @@ extern "C" int tgdn_gated_norm_bwd(const tgdn_rows* host_x, const tgdn_rows* hos
   if (gated && host_gate->type != xt) return TGDN_ERR_TYPE;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   const tgdn_rows dxo = dense(dx, xt, rows, N), dzo = dense(gated ? dgate : nullptr, xt, rows, N);
-  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(xt), {host_x, gated ? host_gate : nullptr, host_dout, &dxo, &dzo}), vec_of(xt));
-  const int blocks = norm_blocks(s, rows);
+  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(xt), {host_x, gated ? host_gate : nullptr, host_dout, &dxo, &dzo}), xt, ot);
+  const int blocks = norm_blocks(s, rows, true);
   const bool want_w = host_dweight && host_dweight->data, want_c = host_dscale && host_dscale->data;
   if ((want_w || want_c) && (!scratch || scratch_floats < static_cast<int64_t>(blocks) * N)) return TGDN_ERR_SCRATCH;
   NormParams p = norm_params(rows, N, 0.f, s, host_weight, host_scale, scale_value);

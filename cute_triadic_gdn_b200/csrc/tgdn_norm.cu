@@ -4,8 +4,8 @@
 namespace tgdn {
 
 template <typename TX, typename TR, int VEC, bool EDGES, int SIZE>
-__global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 3 : 1) residual_fwd_kernel(NormParams p) {
-  constexpr int E = NORM_CHANNELS, K = E / VEC;
+__global__ void TGDN_NORM_BOUNDS(false) residual_fwd_kernel(NormParams p) {
+  constexpr int E = norm_channels(sizeof(TX), SIZE), K = E / VEC;
   extern __shared__ float4 vectors[];
   __shared__ float red[2][NORM_MAX_WARPS];
   Walk<VEC, K, EDGES> walk(p);
@@ -46,8 +46,8 @@ __global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 3 : 
 }
 
 template <typename TX, typename TR, int VEC, bool EDGES, int SIZE>
-__global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 2 : 1) residual_bwd_kernel(NormParams p) {
-  constexpr int E = NORM_CHANNELS, K = E / VEC;
+__global__ void TGDN_NORM_BOUNDS(true) residual_bwd_kernel(NormParams p) {
+  constexpr int E = norm_channels(sizeof(TX), SIZE), K = E / VEC;
   extern __shared__ float4 vectors[];
   __shared__ float red[2][NORM_MAX_WARPS];
   Walk<VEC, K, EDGES> walk(p);
@@ -75,7 +75,16 @@ __global__ void __launch_bounds__(norm_threads(SIZE), SIZE == NORM_GROUPS ? 2 : 
   for (int phase = 0; walk.base < p.rows; walk.base += walk.step, phase ^= 1) {
     const int64_t row = walk.row();
     const bool ok = row < p.rows;
-    if (!AHEAD) request(row);
+    if (!AHEAD) {
+      request(row);
+      if (threadIdx.x == 0 && row + walk.step < p.rows) {
+        const uint32_t r = static_cast<uint32_t>(row + walk.step);
+        pull_row(static_cast<const TR*>(p.stream) + r * static_cast<int64_t>(p.N), p.N);
+        if (p.dy.p) pull_row(static_cast<const TX*>(p.dy.p) + p.dy.at(r), p.N);
+        if (p.dstream.p) pull_row(static_cast<const TR*>(p.dstream.p) + p.dstream.at(r), p.N);
+        if (p.sums1) pull_row(static_cast<const TX*>(p.x.p) + p.x.at(r), p.N);
+      }
+    }
     Row<E> n = nr.get(walk.cols), dy = yr.get(walk.cols), ds = sr.get(walk.cols), x;
     if (p.sums1) x = xr.get(walk.cols);
     const float inv = next_inv;
@@ -120,6 +129,7 @@ __global__ void __launch_bounds__(32 * SUM_ROWS) norm_sums_kernel(SumParams p) {
   const int j = threadIdx.x & 31, i = threadIdx.x >> 5, c = blockIdx.x * 32 + j;
   float s = 0.f;
   if (c < p.N)
+#pragma unroll 8
     for (int b = i; b < p.blocks; b += SUM_ROWS) s += p.partials[static_cast<int64_t>(b) * p.N + c];
   part[i][j] = s;
   __syncthreads();
@@ -150,12 +160,12 @@ TGDN_LAUNCHER(ResidualBwd, residual_bwd_kernel);
 extern "C" int64_t tgdn_norm_scratch_floats(int64_t rows, int N) {
   if (check_norm(rows, N)) return 0;
   int most = 0;
-  for (const int vec : {4, 8}) {                  // whichever layout the alignment allows
-    for (const bool vectors : {true, false}) {
-      const int b = norm_blocks(norm_shape(N, vectors, vec), rows);
-      if (b > most) most = b;
-    }
-  }
+  for (const int x_type : {TGDN_F32, TGDN_BF16})         // whichever types and layout the call comes with
+    for (const int other : {TGDN_F32, TGDN_BF16})
+      for (const bool vectors : {true, false}) {
+        const int b = norm_blocks(norm_shape(N, vectors, x_type, other), rows, true);
+        if (b > most) most = b;
+      }
   return 2 * static_cast<int64_t>(most) * N;
 }
 
@@ -168,10 +178,10 @@ extern "C" int tgdn_residual_norm_fwd(const tgdn_rows* host_x, const tgdn_rows* 
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   const int xt = host_x->type, rt = host_residual->type;
   const tgdn_rows yo = dense(y, xt, rows, N), so = dense(stream_out, rt, rows, N);
-  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(xt), {host_x, host_residual, &yo, &so}), vec_of(xt));
+  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(xt), {host_x, host_residual, &yo, &so}), xt, rt);
   NormParams p = norm_params(rows, N, eps, s, host_weight, host_scale, scale_value);
   p.x = rows_at(host_x, rows); p.other = rows_at(host_residual, rows); p.out = y; p.stream = stream_out; p.rstd = rstd;
-  return launch_types<ResidualFwd>(xt, rt, s, norm_blocks(s, rows), p, static_cast<cudaStream_t>(stream));
+  return launch_types<ResidualFwd>(xt, rt, s, norm_blocks(s, rows, false), p, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tgdn_residual_norm_bwd(const void* stream_in, int stream_type, const tgdn_rows* host_x, int x_type, const tgdn_rows* host_dy,
@@ -190,8 +200,8 @@ extern "C" int tgdn_residual_norm_bwd(const void* stream_in, int stream_type, co
   if ((host_dy && host_dy->data && host_dy->type != x_type) || (host_dstream && host_dstream->data && host_dstream->type != stream_type)) return TGDN_ERR_TYPE;
   if (!tgdn_check_device()) return TGDN_ERR_DEVICE;
   const tgdn_rows si = dense(stream_in, stream_type, rows, N), dr = dense(dresidual, stream_type, rows, N), dxo = dense(dx, x_type, rows, N);
-  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(x_type), {&si, &dr, &dxo, host_dy, host_dstream, want_c ? host_x : nullptr}), vec_of(x_type));
-  const int blocks = norm_blocks(s, rows);
+  const NormShape s = norm_shape(N, vectors_ok(rows, N, vec_of(x_type), {&si, &dr, &dxo, host_dy, host_dstream, want_c ? host_x : nullptr}), x_type, stream_type);
+  const int blocks = norm_blocks(s, rows, true);
   if ((want_w || want_c) && (!scratch || scratch_floats < 2 * static_cast<int64_t>(blocks) * N)) return TGDN_ERR_SCRATCH;
   NormParams p = norm_params(rows, N, 0.f, s, host_weight, host_scale, scale_value);
   p.x = rows_at(want_c ? host_x : nullptr, rows); p.dy = rows_at(host_dy, rows); p.dstream = rows_at(host_dstream, rows);

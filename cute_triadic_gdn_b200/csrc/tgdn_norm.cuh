@@ -28,9 +28,19 @@ namespace tgdn {
 
 constexpr int NORM_BLOCK = 256;                  // threads of a block that holds several rows
 constexpr int NORM_MAX_WARPS = 32;
-constexpr int NORM_CHANNELS = 16;                 // of a row, a thread
-enum NormSize { NORM_GROUPS, NORM_WIDE, NORM_WIDEST };   // several rows a block; one row, up to 512 threads; up to 1024
-constexpr int norm_threads(int size) { return size == NORM_GROUPS ? NORM_BLOCK : size == NORM_WIDE ? 512 : 1024; }
+// How rows lie on blocks: several a block, or one a block of up to 512 or of up to 1024 threads.
+enum NormSize { NORM_GROUPS, NORM_WIDE, NORM_WIDEST };
+// Channels of a row a thread.  Sixteen, but for short rows of 32 bits, which would not fit the registers beside the next row's.
+constexpr int norm_channels(int bytes, int size) { return bytes == 4 && size == NORM_GROUPS ? 8 : 16; }
+// Threads of a block, and blocks an SM, that a kernel's registers are sized for: as many bytes on their way as possible without spilling.
+// Forward, rows of up to 512 threads: 80 registers do where both types have 16 bits (65536 x 2048, gated: 193 us with 100 registers, 150
+// with 80), not with a stream in 32 bits (32768 x 4096: 250 and 293 us).
+constexpr int norm_threads(int size, bool backward, bool small) {
+  return size == NORM_GROUPS ? NORM_BLOCK : size == NORM_WIDEST ? 1024 : backward || !small ? 512 : 768;
+}
+constexpr int norm_blocks_of(int size, bool backward, bool small) { return size != NORM_GROUPS ? 1 : backward || !small ? 2 : 3; }
+#define TGDN_NORM_BOUNDS(backward)                                                                    \
+  __launch_bounds__(norm_threads(SIZE, backward, sizeof(TX) + sizeof(TR) == 4), norm_blocks_of(SIZE, backward, sizeof(TX) + sizeof(TR) == 4))
 
 struct RowsAt {                                  // row r of the tensor starts at (r / inner) * so + (r % inner) * si
   const void* p;
@@ -139,10 +149,16 @@ __device__ __forceinline__ void store_row(T* row, bool ok, const Columns<VEC, K,
 template <int VEC, int K, bool EDGES>
 __device__ __forceinline__ Row<K * VEC> load_small(const SmallVector& s, float otherwise, const Columns<VEC, K, EDGES>& cols) {
   Row<K * VEC> r;
+  auto take = [&](auto get) {
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) r.v[k * VEC + i] = cols.holds(cols.at(k) + i) ? s.get(cols.at(k) + i, otherwise) : 0.f;
+      for (int i = 0; i < VEC; ++i) r.v[k * VEC + i] = cols.holds(cols.at(k) + i) ? get(cols.at(k) + i) : 0.f;
+  };
+  if (!s.p) take([&](int) { return otherwise; });
+  else if (s.type == TGDN_F32) take([&](int i) { return static_cast<const float*>(s.p)[i]; });
+  else if (s.type == TGDN_BF16) take([&](int i) { return to_f32(static_cast<const __nv_bfloat16*>(s.p)[i]); });
+  else take([&](int i) { return to_f32(static_cast<const __half*>(s.p)[i]); });
   return r;
 }
 
@@ -180,6 +196,13 @@ struct Walk {
         cols(lane, p.tpr, EDGES ? static_cast<int>((base + group) * p.N % VEC) : 0, p.N) {}
   __device__ __forceinline__ int64_t row() const { return base + group; }
 };
+
+// Asks for a row of the next round, on its way into L2 while this one is worked on (one thread; whole 16-byte pieces inside the row).
+template <typename T>
+__device__ __forceinline__ void pull_row(const T* row, int N) {
+  const uintptr_t from = (reinterpret_cast<uintptr_t>(row) + 15) & ~static_cast<uintptr_t>(15), to = reinterpret_cast<uintptr_t>(row + N) & ~static_cast<uintptr_t>(15);
+  if (to > from) bulk_prefetch(reinterpret_cast<const void*>(from), static_cast<uint32_t>(to - from));
+}
 
 // Sum over the `tpr` threads of a row; every one of them gets it.  Rows of several warps are one per block: `red` is double-buffered by
 // the caller (`phase`), so one barrier a sum is enough.
@@ -235,35 +258,47 @@ int norm_add_up(const float* partials, int blocks, int N, const tgdn_vector* f0,
 namespace tgdn {
 namespace {
 
-// How a row is laid over threads: `tpr` threads of sixteen channels each, a power of two of a warp's lanes as far as they go and whole warps
-// beyond.
+// How a row is laid over threads: `tpr` threads, a power of two of a warp's lanes as far as they go and whole warps beyond.
 struct NormShape {
-  int vec, tpr, threads, groups;
-  bool edges;
+  int vec, tpr, threads, groups, size;
+  bool edges, small;
 };
-NormShape norm_shape(int N, bool vectors, int vec_elements) {
+NormShape norm_shape(int N, bool vectors, int x_type, int other_type) {
   NormShape s;
-  s.vec = vectors ? vec_elements : 1;
+  const int bytes = type_bytes(x_type);
+  s.small = bytes + type_bytes(other_type) == 4;
+  s.vec = vectors ? 16 / bytes : 1;
   s.edges = N % s.vec != 0;
-  const int units = (N + (s.edges ? s.vec - 1 : 0) + s.vec - 1) / s.vec, need = (units * s.vec + NORM_CHANNELS - 1) / NORM_CHANNELS;
-  if (need <= 32) {
+  const int units = (N + (s.edges ? s.vec - 1 : 0) + s.vec - 1) / s.vec * s.vec;
+  const int few = (units + norm_channels(bytes, NORM_GROUPS) - 1) / norm_channels(bytes, NORM_GROUPS), many = (units + 15) / 16;
+  if (few <= 32) {
+    s.size = NORM_GROUPS;
     s.tpr = 1;
-    while (s.tpr < need) s.tpr *= 2;
+    while (s.tpr < few) s.tpr *= 2;
     s.threads = NORM_BLOCK;
   } else {
-    s.tpr = (need + 31) / 32 * 32;
-    s.threads = s.tpr;
+    s.tpr = s.threads = (many + 31) / 32 * 32;
+    s.size = s.threads <= 512 ? NORM_WIDE : NORM_WIDEST;
   }
-  if (s.threads > 1024) return norm_shape(N, false, vec_elements);     // (the widest rows, where they do not start on a vector's border)
+  if (s.threads > 1024) return norm_shape(N, false, x_type, other_type);     // (the widest rows, where they do not start on a vector's border)
   s.groups = s.threads / s.tpr;
   return s;
 }
 
-// Blocks of a pass: as many as hold the rows, at most two thousand threads' worth on every SM; rows of a group are multiples of eight apart.
-int norm_blocks(const NormShape& s, int64_t rows) {
-  const int64_t want = (rows + s.groups - 1) / s.groups, most = static_cast<int64_t>(tgdn_sm_count()) * (2048 / s.threads > 0 ? 2048 / s.threads : 1);
-  const int multiple = s.groups >= 8 ? 1 : 8 / s.groups;
-  return static_cast<int>(((want < most ? want : most) + multiple - 1) / multiple * multiple);
+// Blocks of a pass: as many as hold the rows, at most what the SMs hold at once (a block fetches the vectors over the channels first and
+// leaves a partial of its sums last: 3000 rows of 2001 channels in 2368 blocks took 47 us backward, in 500 blocks 28), in whole rounds of
+// equal length.  Where a block would walk 32 rows and more it takes a quarter of them and leaves the SMs to even out (forward, 32768 x 4096
+// with an f32 stream: 264 -> 248 us; heads of 128 in 32 bits, backward: 442 -> 409 us); backward, one row a block, the partials cost what
+// that gains (bf16, 32768 x 4096: 190 -> 210 us), and half is right with 32 bits (446 -> 420 us).  Rows of a group are multiples of eight
+// apart.
+int norm_blocks(const NormShape& s, int64_t rows, bool backward) {
+  const int64_t want = (rows + s.groups - 1) / s.groups;
+  const int per_sm = norm_blocks_of(s.size, backward, s.small) * (norm_threads(s.size, backward, s.small) / s.threads);
+  int64_t most = static_cast<int64_t>(tgdn_sm_count()) * per_sm;
+  if (want >= most * 32) most *= !backward || s.size == NORM_GROUPS ? 4 : s.small ? 1 : 2;
+  const int64_t rounds = (want + most - 1) / most;
+  const int multiple = !s.edges || s.groups >= 8 ? 1 : 8 / s.groups;
+  return static_cast<int>(((want + rounds - 1) / rounds + multiple - 1) / multiple * multiple);
 }
 
 // True when the rows can be moved as vectors: every row starts as far behind a vector's border as row * N elements do, and what a vector
@@ -303,11 +338,11 @@ int check_vector(const tgdn_vector* v) { return v && v->data && !type_known(v->t
 #define TGDN_TRY(expr) do { if (const int rc_ = (expr)) return rc_; } while (0)
 
 // The kernels by shape: 16-byte vectors (eight channels of 16 bits, four of 32), the same with rows that start inside one, or single
-// channels; several rows a block, one of up to 512 threads or one of up to 1024 (whose registers differ).
+// channels, in the three sizes.
 template <typename TX, typename TR, int VEC, bool EDGES, template <typename, typename, int, bool, int> class Launch>
 int launch_size(const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {
-  if (s.tpr <= 32) return Launch<TX, TR, VEC, EDGES, NORM_GROUPS>::go(s, blocks, p, st);
-  return s.threads <= 512 ? Launch<TX, TR, VEC, EDGES, NORM_WIDE>::go(s, blocks, p, st) : Launch<TX, TR, VEC, EDGES, NORM_WIDEST>::go(s, blocks, p, st);
+  if (s.size == NORM_GROUPS) return Launch<TX, TR, VEC, EDGES, NORM_GROUPS>::go(s, blocks, p, st);
+  return s.size == NORM_WIDE ? Launch<TX, TR, VEC, EDGES, NORM_WIDE>::go(s, blocks, p, st) : Launch<TX, TR, VEC, EDGES, NORM_WIDEST>::go(s, blocks, p, st);
 }
 template <typename TX, typename TR, template <typename, typename, int, bool, int> class Launch>
 int launch_shape(const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {
@@ -318,8 +353,8 @@ int launch_shape(const NormShape& s, int blocks, const NormParams& p, cudaStream
 // Dynamic shared memory: two vectors over the channels (which the sums over a block's groups use after them).
 template <typename Kernel>
 int launch_norm(Kernel kernel, bool* configured, const NormShape& s, int blocks, const NormParams& p, cudaStream_t st) {
-  const int bytes = 2 * NORM_CHANNELS * 4 * s.threads;
-  if (const int rc = tgdn_dynamic_smem(reinterpret_cast<const void*>(kernel), 2 * NORM_CHANNELS * 4 * 1024, configured)) return rc;
+  const int bytes = 2 * 16 * 4 * s.threads;
+  if (const int rc = tgdn_dynamic_smem(reinterpret_cast<const void*>(kernel), 2 * 16 * 4 * 1024, configured)) return rc;
   kernel<<<blocks, s.threads, bytes, st>>>(p);
   return tgdn_cuda_error(cudaGetLastError());
 }
