@@ -40,9 +40,10 @@ SIGNATURES = {
     "tgdn_bwd_state_grads": (_I, [_P] * 10 + [_F, _P] + [_I] * 5 + [_P] * 5),
     "tgdn_bwd_matrix": (_I, [_P] * 16 + [_F, _P] + [_I] * 5 + [_P] * 7),
     "tgdn_scan_carry_floats": (_L, [_I, _I, _I]),
+    "tgdn_scan_scratch_floats": (_L, [_I, _I, _I]),
     "tgdn_scan_map": (_I, [_P, _I, _I, _I, _P, _P, _P]),
-    "tgdn_scan_fwd": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
-    "tgdn_scan_bwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I] + [_P] * 7),
+    "tgdn_scan_fwd": (_I, [_P, _P, _P, _I, _I, _I, _I] + [_P] * 5 + [_L, _P]),
+    "tgdn_scan_bwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I] + [_P] * 7 + [_L, _P]),
     "tgdn_scan_step": (_I, [_P, _P, _I, _I, _P, _P, _P]),
     "tgdn_norm_scratch_floats": (_L, [_L, _I]),
     "tgdn_residual_norm_fwd": (_I, [_P, _P, _P, _P, _F, _L, _I, _F, _P, _P, _P, _P]),

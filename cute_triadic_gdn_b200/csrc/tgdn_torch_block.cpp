@@ -74,6 +74,11 @@ std::tuple<Tensor, Tensor> scan_map(const Tensor& cu, int64_t tokens) {
   return {map, valid};
 }
 
+Tensor scan_scratch(const Tensor& x) {
+  const int64_t floats = tgdn_scan_scratch_floats(static_cast<int>(x.size(0)), static_cast<int>(x.size(1)), static_cast<int>(x.size(2)));
+  return floats > 0 ? empty({floats}, x, at::kFloat) : Tensor();
+}
+
 // (h, final state, the state before every tile): the last two are empty unless asked for.
 std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& x, const Tensor& g, const OptTensor& initial, const OptTensor& map, int64_t documents,
                                             bool output_final_state, bool save) {
@@ -85,8 +90,10 @@ std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& x, const Tensor& g, co
   if (output_final_state) final_state = empty({has(map) ? documents : x.size(0), x.size(2)}, x, at::kFloat);
   if (save) carry = empty({tgdn_scan_carry_floats(B, T, D)}, x, at::kFloat);
   if (has(initial)) start = initial->contiguous();
+  const Tensor scratch = scan_scratch(x);
   check_rc(tgdn_scan_fwd(&xr.rows, &gr.rows, ptr<int32_t>(map), static_cast<int>(documents), B, T, D, ptr<float>(start), ptr(h),
-                         output_final_state ? ptr<float>(final_state) : nullptr, save ? ptr<float>(carry) : nullptr, stream_of(x)),
+                         output_final_state ? ptr<float>(final_state) : nullptr, save ? ptr<float>(carry) : nullptr, ptr<float>(scratch), scratch.defined() ? scratch.numel() : 0,
+                         stream_of(x)),
            "tgdn_scan_fwd");
   return {h, final_state, carry};
 }
@@ -113,8 +120,10 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(const Tensor& x, const Tensor& g, co
     dinitial = empty({sequences, x.size(2)}, x, at::kFloat);
   }
   if (has(dfinal)) end = dfinal->contiguous();
+  const Tensor scratch = scan_scratch(x);
   check_rc(tgdn_scan_bwd(&xr.rows, &gr.rows, &hr.rows, ptr<int32_t>(map), static_cast<int>(documents), B, T, D, ptr<float>(start),
-                         ptr<float>(carry), ptr<float>(end), ptr(dx), ptr(dg), has(initial) ? ptr<float>(dinitial) : nullptr, stream_of(x)),
+                         ptr<float>(carry), ptr<float>(end), ptr(dx), ptr(dg), has(initial) ? ptr<float>(dinitial) : nullptr, ptr<float>(scratch),
+                         scratch.defined() ? scratch.numel() : 0, stream_of(x)),
            "tgdn_scan_bwd");
   return {dx, dg, dinitial};
 }

@@ -229,15 +229,17 @@ typedef struct {
  * h: (B, T, D) contiguous, x's type. */
 #define TGDN_SCAN_TILE 128
 int64_t tgdn_scan_carry_floats(int B, int T, int D);
+int64_t tgdn_scan_scratch_floats(int B, int T, int D);   /* of the two calls below; 0: none, scratch may be NULL */
 int tgdn_scan_map(const void* cu_seqlens, int cu_is_int64, int n_docs, int T, int32_t* map, uint8_t* valid, void* stream);
 int tgdn_scan_fwd(const tgdn_rows* host_x, const tgdn_rows* host_g, const int32_t* map, int n_docs, int B, int T, int D,
-                  const float* initial, void* h, float* final_state, float* carry, void* stream);
+                  const float* initial, void* h, float* final_state, float* carry, float* scratch, int64_t scratch_floats,
+                  void* stream);
 
 /* The gradients: dh (x's type) and dfinal (f32 (sequences, D), or NULL: zero) -> dx, dg (contiguous, the types of x and g) and, where
  * dinitial is not NULL, dinitial (f32 (sequences, D)). */
 int tgdn_scan_bwd(const tgdn_rows* host_x, const tgdn_rows* host_g, const tgdn_rows* host_dh, const int32_t* map, int n_docs, int B,
                   int T, int D, const float* initial, const float* carry, const float* dfinal, void* dx, void* dg, float* dinitial,
-                  void* stream);
+                  float* scratch, int64_t scratch_floats, void* stream);
 
 /* One token of B sequences on a resident state: state (B, D) f32 <- exp(g) state + x in place, h (B, D) = the new state in x's type.
  * x, g: (B, 1, D). */

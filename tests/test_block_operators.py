@@ -58,13 +58,14 @@ def test_arguments_of_the_c_abi_are_checked_before_a_launch():
     L, fake, null = _lib.lib, ctypes.c_void_p(4096), None
     rows = lambda t=1, data=4096, inner=8: ctypes.byref(_lib.Rows(data, inner, 64, 8, t))
     vec = lambda t=1, data=4096: ctypes.byref(_lib.Vector(data, t))
-    assert L.tgdn_scan_fwd(null, rows(), null, 0, 1, 8, 8, null, fake, null, null, null) == -2
-    assert L.tgdn_scan_fwd(rows(), rows(), null, 0, 1, 8, 8, null, null, null, null, null) == -2
-    assert L.tgdn_scan_fwd(rows(), rows(7), null, 0, 1, 8, 8, null, fake, null, null, null) == -8
-    assert L.tgdn_scan_fwd(rows(), rows(), null, 0, 1, 0, 8, null, fake, null, null, null) == -1
-    assert L.tgdn_scan_fwd(rows(), rows(), fake, 2, 2, 8, 8, null, fake, null, null, null) == -1          # a packed row of two batch rows
-    assert L.tgdn_scan_bwd(rows(), rows(), rows(), null, 0, 1, 8, 8, null, null, null, fake, fake, null, null) == -2
-    assert L.tgdn_scan_bwd(rows(), rows(), rows(0), null, 0, 1, 8, 8, null, fake, null, fake, fake, null, null) == -8
+    assert L.tgdn_scan_fwd(null, rows(), null, 0, 1, 8, 8, null, fake, null, null, null, 0, null) == -2
+    assert L.tgdn_scan_fwd(rows(), rows(), null, 0, 1, 8, 8, null, null, null, null, null, 0, null) == -2
+    assert L.tgdn_scan_fwd(rows(), rows(7), null, 0, 1, 8, 8, null, fake, null, null, null, 0, null) == -8
+    assert L.tgdn_scan_fwd(rows(), rows(), null, 0, 1, 0, 8, null, fake, null, null, null, 0, null) == -1
+    assert L.tgdn_scan_fwd(rows(), rows(), fake, 2, 2, 8, 8, null, fake, null, null, null, 0, null) == -1          # a packed row of two batch rows
+    assert L.tgdn_scan_bwd(rows(), rows(), rows(), null, 0, 1, 8, 8, null, null, null, fake, fake, null, null, 0, null) == -2
+    assert L.tgdn_scan_bwd(rows(), rows(), rows(0), null, 0, 1, 8, 8, null, fake, null, fake, fake, null, null, 0, null) == -8
+    assert L.tgdn_scan_fwd(rows(), rows(), null, 0, 1, 4096, 8, null, fake, null, null, null, 0, null) == -5
     assert L.tgdn_scan_step(rows(), rows(), 1, 8, null, fake, null) == -2
     assert L.tgdn_scan_map(fake, 0, 0, 8, fake, fake, null) == -1 and L.tgdn_scan_map(null, 0, 1, 8, fake, fake, null) == -2
     assert L.tgdn_residual_norm_fwd(rows(), rows(), null, null, 1.0, 8, 16385, 1e-6, fake, fake, null, null) == -1

@@ -140,6 +140,29 @@ def test_results_do_not_depend_on_the_batch_or_on_the_widths_around():
     assert torch.equal(narrow, h[..., :33])
 
 
+@pytest.mark.parametrize("D,x_type,g_type", [(64, BF16, F32), (72, F16, F16), (33, F32, F32)])
+def test_long_sequences_alone_and_in_a_wide_batch(D, x_type, g_type):
+    """Few slices of a long sequence are split along time, many are walked whole: the same bits, and those of the definition."""
+    B, T = 120, 1500
+    x, g, initial, dh, dfinal = make(B, T, D, x_type, g_type)
+    assert _lib.lib.tgdn_scan_scratch_floats(B, T, D) == 0 < _lib.lib.tgdn_scan_scratch_floats(2, T, D)
+    leaves = [t.requires_grad_(True) for t in (x, g, initial)]
+    h, final = gated_scan_call(x, g, initial_state=initial, output_final_state=True)
+    grads = torch.autograd.grad((h, final), leaves, (dh, dfinal))
+    part = [t.detach()[7:9].clone() for t in (x, g, initial, dh, dfinal)]
+    hb, fb, gb = run_and_check(*part)
+    for a, r in zip((hb, fb, *gb), (h, final, *grads)):
+        assert torch.equal(a, r[7:9])
+
+
+@pytest.mark.parametrize("x_type,g_type,D", [(BF16, F32, 40), (F16, F16, 7), (F32, F32, 66), (BF16, BF16, 128)])
+def test_long_packed_rows(x_type, g_type, D):
+    cu = [0, 1, 128, 129, 1000, 1024, 1500, 2047, 2048, 2300]
+    x, g, initial, dh, dfinal = make(1, cu[-1], D, x_type, g_type, sequences=len(cu) - 1)
+    run_and_check(x, g, initial, dh, dfinal, cu)
+    run_and_check(x, g, None, dh, dfinal, cu)
+
+
 def test_segments_and_decode_continue_a_sequence():
     B, T, D = 2, 384 + 40, 66
     x, g, initial, dh, dfinal = make(B, T, D, BF16, F32)
