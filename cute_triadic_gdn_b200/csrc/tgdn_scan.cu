@@ -113,12 +113,13 @@ using namespace tgdn;
 
 namespace {
 
-// The way over the tiles, by the size of the problem alone.  A block of the whole way takes about 1.4 us a tile (two a SM: 2.6 us for both);
-// the split way reads two operands twice and has two launches more, about 6 us.  So the tiles of a slice are split where the slices and batch
-// rows leave a third of the SMs without a block and there are enough tiles to make up for the launches.
+// The way over the tiles, by the size of the problem alone.  One block walks a tile in 1.3 us forward and 2 us backward, whatever the slices
+// beside it (bf16, up to one block an SM); the split way's three launches begin at 9 and 11 us and its two passes over the data add 0.015 and
+// 0.019 us a tile and slice.  So the split way is ahead from 6 tiles on for one slice (64 channels x 16384: 163 -> 11 us forward), from 17 for
+// 64 slices (4096 channels x 4096: 44 -> 36 us, x 1024: 12 -> 13 us), and not above 90 (6144 x 4096: 45 and 59 us).
 bool scan_splits(int B, int T, int D) {
-  const int64_t units = static_cast<int64_t>(B) * ((D + 63) / 64);
-  return units * 3 <= tgdn_sm_count() * 2 && T > 8 * SCAN_TILE;
+  const int64_t units = static_cast<int64_t>(B) * ((D + 63) / 64), tiles = (T - 1) / SCAN_TILE + 1, spare = tgdn_sm_count() * 5 / 8 - units;
+  return spare > 0 && tiles * spare > 500;
 }
 // Blocks of the two passes: a few tiles each, enough of them for four rounds over the SMs.
 void scan_spans(ScanParams& p) {

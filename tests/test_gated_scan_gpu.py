@@ -145,7 +145,7 @@ def test_long_sequences_alone_and_in_a_wide_batch(D, x_type, g_type):
     """Few slices of a long sequence are split along time, many are walked whole: the same bits, and those of the definition."""
     B, T = 120, 1500
     x, g, initial, dh, dfinal = make(B, T, D, x_type, g_type)
-    assert _lib.lib.tgdn_scan_scratch_floats(B, T, D) == 0 < _lib.lib.tgdn_scan_scratch_floats(2, T, D)
+    assert _lib.lib.tgdn_scan_scratch_floats(B, T, D) == 0 < _lib.lib.tgdn_scan_scratch_floats(2, T, D)                # (the two ways)
     leaves = [t.requires_grad_(True) for t in (x, g, initial)]
     h, final = gated_scan_call(x, g, initial_state=initial, output_final_state=True)
     grads = torch.autograd.grad((h, final), leaves, (dh, dfinal))
