@@ -6,7 +6,7 @@ namespace tgdn {
 
 // The states between the tiles from the tiles' maps: carry[i] = the state before tile i (REVERSE: behind it), end = the state behind the last
 // (before the first).  A block has 32 channels of a batch row; all warps bring the maps of 64 tiles at a time into shared memory, three
-// lots ahead, and the first walks over them: a fused multiply-add a tile, 1024 tiles of 1024 channels in 14 us.
+// lots ahead, and the first walks over them: a fused multiply-add a tile, 1024 tiles of 1024 channels in 21 us (a fortieth of the forward and backward around it).
 constexpr int FOLD_TILES = 64, FOLD_STAGES = 4, FOLD_THREADS = 256;
 struct FoldStage {
   float A[FOLD_TILES][32], H[FOLD_TILES][32];
@@ -42,6 +42,8 @@ scan_fold_kernel(const float* A, const float* H, const int* cut, const float* st
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   for (int lot = 0; lot < FOLD_STAGES - 1; ++lot) request(lot);
+  float* out = carry + base + static_cast<int64_t>(tile_of(0)) * D;
+  const int64_t step = REVERSE ? -static_cast<int64_t>(D) : D;
   float state = start && active ? start[static_cast<int64_t>(b) * D + c] : 0.f;
   for (int lot = 0; lot < lots; ++lot) {
     asm volatile("cp.async.wait_group %0;" ::"n"(FOLD_STAGES - 2) : "memory");
@@ -50,9 +52,26 @@ scan_fold_kernel(const float* A, const float* H, const int* cut, const float* st
     if (warp == 0 && active) {
       const FoldStage& s = stages[lot % FOLD_STAGES];
       const int n = min(FOLD_TILES, tiles - lot * FOLD_TILES);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        carry[base + static_cast<int64_t>(tile_of(lot * FOLD_TILES + i)) * D] = state;
+      int i = 0;
+      for (; i + 8 <= n; i += 8) {               // eight maps in registers at a time, so that the walk waits for its own sums only
+        float a[8], h[8];
+        int cuts = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          a[k] = s.A[i + k][lane];
+          h[k] = s.H[i + k][lane];
+          if (cut) cuts |= (s.cut[i + k] != 0) << k;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          *out = state;
+          out += step;
+          state = cuts >> k & 1 ? h[k] : fmaf(a[k], state, h[k]);
+        }
+      }
+      for (; i < n; ++i) {
+        *out = state;
+        out += step;
         state = cut && s.cut[i] ? s.H[i][lane] : fmaf(s.A[i][lane], state, s.H[i][lane]);
       }
     }
@@ -116,10 +135,11 @@ namespace {
 // The way over the tiles, by the size of the problem alone.  One block walks a tile in 1.3 us forward and 2 us backward, whatever the slices
 // beside it (bf16, up to one block an SM); the split way's three launches begin at 9 and 11 us and its two passes over the data add 0.015 and
 // 0.019 us a tile and slice.  So the split way is ahead from 6 tiles on for one slice (64 channels x 16384: 163 -> 11 us forward), from 17 for
-// 64 slices (4096 channels x 4096: 44 -> 36 us, x 1024: 12 -> 13 us), and not above 90 (6144 x 4096: 45 and 59 us).
+// 64 slices (4096 channels x 4096: 44 -> 36 us, x 1024: 12 -> 13 us), and not above 90 (6144 x 4096: 45 and 59 us).  Four more launches of a
+// forward and backward cost the host 15 us where it is what a call waits for (3 x 1000 x 333: 69 and 84 us a step): twice the tiles.
 bool scan_splits(int B, int T, int D) {
   const int64_t units = static_cast<int64_t>(B) * ((D + 63) / 64), tiles = (T - 1) / SCAN_TILE + 1, spare = tgdn_sm_count() * 5 / 8 - units;
-  return spare > 0 && tiles * spare > 500;
+  return spare > 0 && tiles * spare > 1000;
 }
 // Blocks of the two passes: a few tiles each, enough of them for four rounds over the SMs.
 void scan_spans(ScanParams& p) {
@@ -152,7 +172,7 @@ bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) %
 
 int scan_checks(const tgdn_rows* x, const tgdn_rows* g, const int32_t* map, int n_docs, int B, int T, int D) {
   if (!x || !g || !x->data || !g->data) return TGDN_ERR_NULL;
-  if (B <= 0 || T <= 0 || T > 0x7fffffff - 2 * SCAN_TILE || D <= 0 || (map && (B != 1 || n_docs <= 0))) return TGDN_ERR_SHAPE;
+  if (B <= 0 || T <= 0 || T > 0x7fffffff - 2 * SCAN_TILE || D <= 0 || D > 0x7fffffff - 64 || (map && (B != 1 || n_docs <= 0))) return TGDN_ERR_SHAPE;
   if (!type_known(x->type) || !type_known(g->type)) return TGDN_ERR_TYPE;
   if (x->stride_inner > 0x7fffffffLL || g->stride_inner > 0x7fffffffLL || x->stride_inner < 0 || g->stride_inner < 0) return TGDN_ERR_SHAPE;
   return 0;

@@ -315,11 +315,12 @@ struct Place {
   int lane, warp, b, slice0, c0, lo, hi;
   bool active;
   int64_t state;                                 // of the lane's first channel in a (sequences, D) tensor's row b
-  __device__ explicit Place(const ScanParams& p) {
+  // `last_first`: the second pass over the data begins where the first one ended, with what L2 still holds.
+  __device__ Place(const ScanParams& p, bool last_first) {
     lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
-    const int unit = blockIdx.x / p.spans, slice = unit % p.slices;
-    lo = (blockIdx.x - unit * p.spans) * p.per_span;
+    const int block = last_first ? gridDim.x - 1 - blockIdx.x : blockIdx.x, unit = block / p.spans, slice = unit % p.slices;
+    lo = (block - unit * p.spans) * p.per_span;
     hi = min(lo + p.per_span, p.tiles);
     b = unit / p.slices;
     slice0 = slice * 32 * VEC;

@@ -13,7 +13,7 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ SharedMaps<VEC, PACKED> maps[STATES ? 2 : 1];     // reverse, forward
   __shared__ RingControl control;
-  const Place<VEC> at(p);
+  const Place<VEC> at(p, WAY == SCAN_FINISH);
   const int lane = at.lane, warp = at.warp, c0 = at.c0;
   const bool active = at.active;
   const int64_t xb = at.b * p.x.sb + (active ? c0 : 0), gb = at.b * p.g.sb + (active ? c0 : 0), hb = at.b * p.dh.sb + (active ? c0 : 0);

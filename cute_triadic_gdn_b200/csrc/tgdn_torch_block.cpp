@@ -30,11 +30,13 @@ void check_sm100(const Tensor& x, const char* call) {
 Tensor none(const Tensor& like) { return at::empty({0}, like.options().dtype(at::kFloat)); }
 
 // ---- gated scan -------------------------------------------------------------------------------------------------------
-// A (B, T, D) tensor as the library reads it; an axis of size one may carry any stride.
+// A (B, T, D) tensor as the library reads it; an axis of size one may carry any stride.  Channels apart, or tokens that are 2^31 elements
+// apart, are copied together.
 struct SequenceRows {
   Tensor held;
   tgdn_rows rows;
-  explicit SequenceRows(const Tensor& t) : held(t.size(2) == 1 || t.stride(2) == 1 ? t : t.contiguous()) {
+  explicit SequenceRows(const Tensor& t)
+      : held((t.size(2) == 1 || t.stride(2) == 1) && (t.size(1) == 1 || t.stride(1) < (int64_t{1} << 31)) ? t : t.contiguous()) {
     rows = {held.data_ptr(), held.size(1), held.size(0) == 1 ? 0 : held.stride(0), held.size(1) == 1 ? 0 : held.stride(1), type_of(held)};
   }
 };

@@ -37,7 +37,7 @@ def run_and_check(x, g, initial, dh, dfinal, cu=None):
 
 
 @pytest.mark.parametrize("x_type,g_type", PAIRS)
-@pytest.mark.parametrize("B,T,D", [(1, 1, 1), (2, 16, 2), (1, 17, 63), (2, 128, 64), (1, 129, 66), (3, 300, 5), (1, 1025, 130)])
+@pytest.mark.parametrize("B,T,D", [(1, 1, 1), (2, 16, 2), (1, 17, 63), (2, 128, 64), (1, 129, 66), (3, 300, 5), (1, 1025, 130), (2, 200, 8), (1, 260, 24)])
 def test_dense_against_the_definition(B, T, D, x_type, g_type):
     x, g, initial, dh, dfinal = make(B, T, D, x_type, g_type)
     run_and_check(x, g, initial, dh, dfinal)
