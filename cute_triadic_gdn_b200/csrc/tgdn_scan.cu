@@ -162,10 +162,10 @@ int scan_fold(const ScanParams& p, bool reverse, const float* start, float* carr
 
 ScanIn scan_in(const tgdn_rows& t, int T) { return {t.data, t.stride_outer, T == 1 ? 0 : static_cast<int>(t.stride_inner)}; }
 
-// What the copy engine takes: rows of whole 16-byte pieces, axes that advance.  Pairs of the outputs follow from D.
+// What the copy engine takes: rows of whole 16-byte pieces that follow one another.  Pairs of the outputs follow from D.
 bool in_pieces(const tgdn_rows& t, int B, int T, int D) {
   const int64_t piece = 16 / type_bytes(t.type);
-  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && D % piece == 0 && (T == 1 || (t.stride_inner > 0 && t.stride_inner % piece == 0)) &&
+  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && D % piece == 0 && (T == 1 || (t.stride_inner >= D && t.stride_inner % piece == 0)) &&
          (B == 1 || (t.stride_outer > 0 && t.stride_outer % piece == 0 && t.stride_outer < int64_t{1} << 36));
 }
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

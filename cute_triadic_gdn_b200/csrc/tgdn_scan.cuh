@@ -60,8 +60,8 @@ struct ScanParams {
   int* status;
 };
 
-// A lane's channels of one row.  Pairs go through the two-wide f32 instructions: the kernels would be bound by the issue of
-// instructions otherwise (one at a time: 37 an element forward, 102 us at 8 x 4096 x 2048 in bf16; see the note at the launch).
+// A lane's channels of one row.  Pairs go through the two-wide f32 instructions: with one channel an instruction the forward issues 37 an
+// element and is bound by that, with two 21 (8 x 4096 x 2048 in bf16, tiles in registers: 102 and 94 us; by the ring 78).
 template <int VEC>
 struct alignas(4 * VEC) Lanes {
   float v[VEC];
@@ -240,8 +240,10 @@ struct alignas(16) SharedMaps {
   __device__ Map<VEC, PACKED> get(int buf, int part, int lane) const { return {A[buf][part][lane], H[buf][part][lane], PACKED ? cut[buf][part] : 0}; }
 };
 
-// The ring of tiles on their way: stages of shared memory that the copy engine fills, each a block's rows of all its inputs, with a barrier
-// that completes when a stage's bytes are in.  One thread asks for a stage again as soon as all warps have what they need of it.
+// The ring of tiles on their way: two to four stages of shared memory that the copy engine fills, each a block's rows of all its inputs, with
+// a barrier that completes when a stage's bytes are in.  One thread asks for a stage again as soon as all warps have what they need of it.
+// 64 to 196 KB of an SM's memory are under way so, where a tile in registers was 32 (8 x 4096 x 2048 in bf16: 94 -> 78 us forward, 174 -> 139
+// backward, of which 63 and 104 are the bytes at the copy rate; 4 x 4096 x 4096 with f32 gates: 129 -> 92 of 84).
 constexpr int SCAN_MAX_STAGES = 4;
 __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int c, int t, int b) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"

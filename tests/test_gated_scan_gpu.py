@@ -114,6 +114,10 @@ def test_strides_are_read_in_place_and_change_nothing():
     for view in (lambda t: wide(t, 8), lambda t: wide(t, 7), by_channel, by_time, shifted):
         for a, b in zip(step(view(x), view(g), view(dh)), ref):
             assert torch.equal(a, b)
+    # windows that overlap: rows that start eight channels after one another
+    flat = torch.cat([x.flatten(), x.flatten()])
+    windows = flat.as_strided((B, T, D), (T * 8, 8, 1))
+    assert torch.equal(gated_scan_call(windows, g), gated_scan_call(windows.contiguous(), g))
     # gates per batch row, expanded over tokens, and per token, expanded over channels; the gradient of a sum is an expanded number
     for shape in ((B, 1, D), (1, T, 1), (1, 1, 1)):
         small = g[:shape[0], :shape[1], :shape[2]].clone().requires_grad_(True)
