@@ -17,8 +17,8 @@ def _like(t, dtype=None):
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
-def _rstd(x):
-    return x.new_empty(x.shape[:-1].numel(), dtype=torch.float32)
+def _rstd(x, save):
+    return x.new_empty(x.shape[:-1].numel() if save else 0, dtype=torch.float32)
 
 
 def _none(x):
@@ -26,8 +26,8 @@ def _none(x):
 
 
 @torch.library.register_fake("tgdn_b200::residual_norm_fwd")
-def _residual_fwd_fake(x, residual, weight, scale, scale_value, eps):
-    return _like(x), _like(residual), _rstd(x)
+def _residual_fwd_fake(x, residual, weight, scale, scale_value, eps, save=False):
+    return _like(x), _like(residual), _rstd(x, save)
 
 
 @torch.library.register_fake("tgdn_b200::residual_norm_bwd")
@@ -38,8 +38,8 @@ def _residual_bwd_fake(stream, x, x_type, dy, dstream, weight, scale, scale_valu
 
 
 @torch.library.register_fake("tgdn_b200::gated_norm_fwd")
-def _gated_fwd_fake(x, gate, weight, residual, scale, scale_value, activation, eps):
-    return _like(x, None if residual is None else residual.dtype), _rstd(x)
+def _gated_fwd_fake(x, gate, weight, residual, scale, scale_value, activation, eps, save=False):
+    return _like(x, None if residual is None else residual.dtype), _rstd(x, save)
 
 
 @torch.library.register_fake("tgdn_b200::gated_norm_bwd")

@@ -3,6 +3,8 @@
 // launches here, the fake implementations in Python beside the calls (gated_scan.py, block_norm.py).
 #include "tgdn_torch.h"
 
+#include <ATen/cuda/EmptyTensor.h>
+
 namespace {
 
 using namespace tgdn_torch;
@@ -27,7 +29,11 @@ void check_sm100(const Tensor& x, const char* call) {
   TORCH_CHECK_VALUE(at::cuda::getDeviceProperties(x.device().index())->major == 10, call, " requires an sm_100 device");
 }
 
-Tensor none(const Tensor& like) { return at::empty({0}, like.options().dtype(at::kFloat)); }
+// Outputs straight from the allocator: a small call is the host's time, and the dispatcher's part of an allocation is half of it.
+Tensor fresh(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+Tensor none(const Tensor& like) { return fresh({0}, like, at::kFloat); }
 
 // ---- gated scan -------------------------------------------------------------------------------------------------------
 // A (B, T, D) tensor as the library reads it; an axis of size one may carry any stride.  Channels apart, or tokens that are 2^31 elements
@@ -69,7 +75,7 @@ std::tuple<Tensor, Tensor> scan_map(const Tensor& cu, int64_t tokens) {
   const c10::cuda::CUDAGuard guard(cu.device());
   TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 2 && cu.is_contiguous() && (cu.scalar_type() == at::kInt || cu.scalar_type() == at::kLong),
                     "cu_seqlens: a contiguous vector of int32 or int64 document offsets, at least [0, T]");
-  Tensor map = empty({tokens}, cu, at::kInt), valid = empty({1}, cu, at::kBool);
+  Tensor map = fresh({tokens}, cu, at::kInt), valid = fresh({1}, cu, at::kBool);
   check_rc(tgdn_scan_map(ptr(cu), cu.scalar_type() == at::kLong ? 1 : 0, static_cast<int>(cu.numel() - 1), static_cast<int>(tokens),
                          ptr<int32_t>(map), ptr<uint8_t>(valid), stream_of(cu)),
            "tgdn_scan_map");
@@ -78,7 +84,7 @@ std::tuple<Tensor, Tensor> scan_map(const Tensor& cu, int64_t tokens) {
 
 Tensor scan_scratch(const Tensor& x) {
   const int64_t floats = tgdn_scan_scratch_floats(static_cast<int>(x.size(0)), static_cast<int>(x.size(1)), static_cast<int>(x.size(2)));
-  return floats > 0 ? empty({floats}, x, at::kFloat) : Tensor();
+  return floats > 0 ? fresh({floats}, x, at::kFloat) : Tensor();
 }
 
 // (h, final state, the state before every tile): the last two are empty unless asked for.
@@ -88,9 +94,9 @@ std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& x, const Tensor& g, co
   const c10::cuda::CUDAGuard guard(x.device());
   const int B = static_cast<int>(x.size(0)), T = static_cast<int>(x.size(1)), D = static_cast<int>(x.size(2));
   const SequenceRows xr(x), gr(g);
-  Tensor h = empty(x.sizes(), x, x.scalar_type()), final_state = none(x), carry = none(x), start;
-  if (output_final_state) final_state = empty({has(map) ? documents : x.size(0), x.size(2)}, x, at::kFloat);
-  if (save) carry = empty({tgdn_scan_carry_floats(B, T, D)}, x, at::kFloat);
+  Tensor h = fresh(x.sizes(), x, x.scalar_type()), final_state = none(x), carry = none(x), start;
+  if (output_final_state) final_state = fresh({has(map) ? documents : x.size(0), x.size(2)}, x, at::kFloat);
+  if (save) carry = fresh({tgdn_scan_carry_floats(B, T, D)}, x, at::kFloat);
   if (has(initial)) start = initial->contiguous();
   const Tensor scratch = scan_scratch(x);
   check_rc(tgdn_scan_fwd(&xr.rows, &gr.rows, ptr<int32_t>(map), static_cast<int>(documents), B, T, D, ptr<float>(start), ptr(h),
@@ -116,10 +122,10 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(const Tensor& x, const Tensor& g, co
                           dfinal->device() == x.device(),
                       "dfinal must be like the final state");
   const SequenceRows xr(x), gr(g), hr(dh);
-  Tensor dx = empty(x.sizes(), x, x.scalar_type()), dg = empty(x.sizes(), x, g.scalar_type()), dinitial = none(x), start, end;
+  Tensor dx = fresh(x.sizes(), x, x.scalar_type()), dg = fresh(x.sizes(), x, g.scalar_type()), dinitial = none(x), start, end;
   if (has(initial)) {
     start = initial->contiguous();
-    dinitial = empty({sequences, x.size(2)}, x, at::kFloat);
+    dinitial = fresh({sequences, x.size(2)}, x, at::kFloat);
   }
   if (has(dfinal)) end = dfinal->contiguous();
   const Tensor scratch = scan_scratch(x);
@@ -216,7 +222,7 @@ Tensor scan_decode(const Tensor& x, const Tensor& g, const Tensor& state) {
   check_sm100(x, "gated_scan_decode");
   const c10::cuda::CUDAGuard guard(x.device());
   const SequenceRows xr(squeeze ? x : x.unsqueeze(1)), gr(squeeze ? g : g.unsqueeze(1));
-  Tensor h = empty(x.sizes(), x, x.scalar_type());
+  Tensor h = fresh(x.sizes(), x, x.scalar_type());
   check_rc(tgdn_scan_step(&xr.rows, &gr.rows, static_cast<int>(B), static_cast<int>(D), ptr<float>(state), ptr(h), stream_of(x)), "tgdn_scan_step");
   return h;
 }
@@ -296,20 +302,22 @@ void check_stream(const Tensor& t, const Tensor& x, const char* name) {
 }
 
 Tensor scratch_for(const Tensor& x, bool wanted) {
-  return wanted ? empty({tgdn_norm_scratch_floats(rows_of(x), static_cast<int>(x.size(-1)))}, x, at::kFloat) : Tensor();
+  return wanted ? fresh({tgdn_norm_scratch_floats(rows_of(x), static_cast<int>(x.size(-1)))}, x, at::kFloat) : Tensor();
 }
 
+// (y, stream, rstd); the last is empty unless a backward follows.
 std::tuple<Tensor, Tensor, Tensor> residual_fwd(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& scale,
-                                                double scale_value, double eps) {
+                                                double scale_value, double eps, bool save) {
   check_norm(x, weight, scale, "residual_norm");
   check_stream(residual, x, "residual");
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t rows = rows_of(x);
   const NormRows xr(x), rr(residual);
   const Vector w(weight), c(scale);
-  Tensor y = empty(x.sizes(), x, x.scalar_type()), stream = empty(x.sizes(), x, residual.scalar_type()), rstd = empty({rows}, x, at::kFloat);
+  Tensor y = fresh(x.sizes(), x, x.scalar_type()), stream = fresh(x.sizes(), x, residual.scalar_type()),
+         rstd = fresh({save ? rows : 0}, x, at::kFloat);
   check_rc(tgdn_residual_norm_fwd(&xr.rows, &rr.rows, &w.v, &c.v, static_cast<float>(scale_value), rows, static_cast<int>(x.size(-1)),
-                                  static_cast<float>(eps), ptr(y), ptr(stream), ptr<float>(rstd), stream_of(x)),
+                                  static_cast<float>(eps), ptr(y), ptr(stream), save ? ptr<float>(rstd) : nullptr, stream_of(x)),
            "tgdn_residual_norm_fwd");
   return {y, stream, rstd};
 }
@@ -334,9 +342,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> residual_bwd(const Tensor& stream, co
   const NormRows xr(want_scale ? x : OptTensor()), yr(dy), sr(dstream);
   const Vector w(weight), c(scale);
   const bool same = !has(scale) && scale_value == 1.0 && x_type == stream.scalar_type();
-  Tensor dresidual = empty(stream.sizes(), stream, stream.scalar_type()), dx = same ? none(stream) : empty(stream.sizes(), stream, x_type);
-  Tensor dweight = want_weight ? empty(weight->sizes(), stream, weight->scalar_type()) : none(stream);
-  Tensor dscale = want_scale ? empty(scale->sizes(), stream, scale->scalar_type()) : none(stream);
+  Tensor dresidual = fresh(stream.sizes(), stream, stream.scalar_type()), dx = same ? none(stream) : fresh(stream.sizes(), stream, x_type);
+  Tensor dweight = want_weight ? fresh(weight->sizes(), stream, weight->scalar_type()) : none(stream);
+  Tensor dscale = want_scale ? fresh(scale->sizes(), stream, scale->scalar_type()) : none(stream);
   const Vector dw(want_weight ? OptTensor(dweight) : OptTensor()), dc(want_scale ? OptTensor(dscale) : OptTensor());
   const Tensor scratch = scratch_for(stream, want_weight || want_scale);
   const int xt = x_type == at::kFloat ? TGDN_F32 : x_type == at::kBFloat16 ? TGDN_BF16 : x_type == at::kHalf ? TGDN_F16 : -1;
@@ -347,8 +355,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> residual_bwd(const Tensor& stream, co
   return {dresidual, dx, dweight, dscale};
 }
 
+// (out, rstd); the last is empty unless a backward follows.
 std::tuple<Tensor, Tensor> gated_fwd(const Tensor& x, const OptTensor& gate, const OptTensor& weight, const OptTensor& residual,
-                                     const OptTensor& scale, double scale_value, int64_t activation, double eps) {
+                                     const OptTensor& scale, double scale_value, int64_t activation, double eps, bool save) {
   check_norm(x, weight, scale, "gated_norm");
   TORCH_CHECK_VALUE(has(gate) == (activation != TGDN_ACT_NONE), "gated_norm: a gate comes with an activation");
   if (has(gate)) {
@@ -361,9 +370,9 @@ std::tuple<Tensor, Tensor> gated_fwd(const Tensor& x, const OptTensor& gate, con
   const int64_t rows = rows_of(x);
   const NormRows xr(x), zr(gate), rr(residual);
   const Vector w(weight), c(scale);
-  Tensor out = empty(x.sizes(), x, has(residual) ? residual->scalar_type() : x.scalar_type()), rstd = empty({rows}, x, at::kFloat);
+  Tensor out = fresh(x.sizes(), x, has(residual) ? residual->scalar_type() : x.scalar_type()), rstd = fresh({save ? rows : 0}, x, at::kFloat);
   check_rc(tgdn_gated_norm_fwd(&xr.rows, &zr.rows, static_cast<int>(activation), &w.v, &rr.rows, &c.v, static_cast<float>(scale_value), rows,
-                               static_cast<int>(x.size(-1)), static_cast<float>(eps), ptr(out), type_of(out), ptr<float>(rstd), stream_of(x)),
+                               static_cast<int>(x.size(-1)), static_cast<float>(eps), ptr(out), type_of(out), save ? ptr<float>(rstd) : nullptr, stream_of(x)),
            "tgdn_gated_norm_fwd");
   return {out, rstd};
 }
@@ -384,9 +393,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_bwd(const Tensor& x, const OptT
   const c10::cuda::CUDAGuard guard(x.device());
   const NormRows xr(x), zr(gate), yr(dout);
   const Vector w(weight), c(scale);
-  Tensor dx = empty(x.sizes(), x, x.scalar_type()), dgate = has(gate) ? empty(x.sizes(), x, x.scalar_type()) : none(x);
-  Tensor dweight = want_weight ? empty(weight->sizes(), x, weight->scalar_type()) : none(x);
-  Tensor dscale = want_scale ? empty(scale->sizes(), x, scale->scalar_type()) : none(x);
+  Tensor dx = fresh(x.sizes(), x, x.scalar_type()), dgate = has(gate) ? fresh(x.sizes(), x, x.scalar_type()) : none(x);
+  Tensor dweight = want_weight ? fresh(weight->sizes(), x, weight->scalar_type()) : none(x);
+  Tensor dscale = want_scale ? fresh(scale->sizes(), x, scale->scalar_type()) : none(x);
   const Vector dw(want_weight ? OptTensor(dweight) : OptTensor()), dc(want_scale ? OptTensor(dscale) : OptTensor());
   const Tensor scratch = scratch_for(x, want_weight || want_scale);
   check_rc(tgdn_gated_norm_bwd(&xr.rows, &zr.rows, static_cast<int>(activation), &yr.rows, &w.v, &c.v, static_cast<float>(scale_value),
@@ -398,14 +407,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_bwd(const Tensor& x, const OptT
 
 using Three = std::tuple<Tensor, Tensor, Tensor>;
 using Two = std::tuple<Tensor, Tensor>;
-Three call_residual_fwd(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& scale, double scale_value, double eps) {
+Three call_residual_fwd(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& scale, double scale_value, double eps,
+                        bool save) {
   static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("tgdn_b200::residual_norm_fwd", "").typed<decltype(residual_fwd)>();
-  return op.call(x, residual, weight, scale, scale_value, eps);
+  return op.call(x, residual, weight, scale, scale_value, eps, save);
 }
 Two call_gated_fwd(const Tensor& x, const OptTensor& gate, const OptTensor& weight, const OptTensor& residual, const OptTensor& scale,
-                   double scale_value, int64_t activation, double eps) {
+                   double scale_value, int64_t activation, double eps, bool save) {
   static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("tgdn_b200::gated_norm_fwd", "").typed<decltype(gated_fwd)>();
-  return op.call(x, gate, weight, residual, scale, scale_value, activation, eps);
+  return op.call(x, gate, weight, residual, scale, scale_value, activation, eps, save);
 }
 
 bool wants_grad(const OptTensor& t) { return has(t) && at::GradMode::is_enabled() && t->requires_grad(); }
@@ -414,7 +424,7 @@ struct ResidualSteps {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& scale,
                                double scale_value, double eps, bool want_weight, bool want_scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, stream, rstd] = call_residual_fwd(x, residual, weight, scale, scale_value, eps);
+    auto [y, stream, rstd] = call_residual_fwd(x, residual, weight, scale, scale_value, eps, true);
     ctx->save_for_backward({stream, rstd, or_undefined(weight), or_undefined(scale), want_scale ? x : Tensor()});
     ctx->saved_data["value"] = scale_value;
     ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
@@ -443,10 +453,11 @@ struct ResidualSteps {
 };
 using ResidualFunction = Differentiable<ResidualSteps>;
 
-Three residual_fwd_autograd(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& scale, double scale_value, double eps) {
+Three residual_fwd_autograd(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& scale, double scale_value, double eps,
+                            bool save) {
   if (!any_grad({&x, &residual}) && !wants_grad(weight) && !wants_grad(scale)) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return call_residual_fwd(x, residual, weight, scale, scale_value, eps);
+    return call_residual_fwd(x, residual, weight, scale, scale_value, eps, save);
   }
   variable_list o = ResidualFunction::apply(x, residual, weight, scale, scale_value, eps, wants_grad(weight), wants_grad(scale));
   return {o[0], o[1], o[2]};
@@ -456,7 +467,7 @@ struct GatedSteps {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& gate, const OptTensor& weight, const OptTensor& residual,
                                const OptTensor& scale, double scale_value, int64_t activation, double eps, bool want_weight, bool want_scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, rstd] = call_gated_fwd(x, gate, weight, residual, scale, scale_value, activation, eps);
+    auto [out, rstd] = call_gated_fwd(x, gate, weight, residual, scale, scale_value, activation, eps, true);
     ctx->save_for_backward({x, rstd, or_undefined(gate), or_undefined(weight), or_undefined(scale)});
     ctx->saved_data["value"] = scale_value;
     ctx->saved_data["activation"] = activation;
@@ -486,23 +497,23 @@ struct GatedSteps {
 using GatedFunction = Differentiable<GatedSteps>;
 
 Two gated_fwd_autograd(const Tensor& x, const OptTensor& gate, const OptTensor& weight, const OptTensor& residual, const OptTensor& scale,
-                       double scale_value, int64_t activation, double eps) {
+                       double scale_value, int64_t activation, double eps, bool save) {
   if (!any_grad({&x}) && !wants_grad(gate) && !wants_grad(weight) && !wants_grad(residual) && !wants_grad(scale)) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return call_gated_fwd(x, gate, weight, residual, scale, scale_value, activation, eps);
+    return call_gated_fwd(x, gate, weight, residual, scale, scale_value, activation, eps, save);
   }
   variable_list o = GatedFunction::apply(x, gate, weight, residual, scale, scale_value, activation, eps, wants_grad(weight), wants_grad(scale));
   return {o[0], o[1]};
 }
 
 Two residual_call(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& scale, double scale_value, double eps) {
-  auto [y, stream, rstd] = call_residual_fwd(x, residual, weight, scale, scale_value, eps);
+  auto [y, stream, rstd] = call_residual_fwd(x, residual, weight, scale, scale_value, eps, false);
   return {y, stream};
 }
 
 Tensor gated_call(const Tensor& x, const OptTensor& gate, const OptTensor& weight, const OptTensor& residual, const OptTensor& scale,
                   double scale_value, int64_t activation, double eps) {
-  return std::get<0>(call_gated_fwd(x, gate, weight, residual, scale, scale_value, activation, eps));
+  return std::get<0>(call_gated_fwd(x, gate, weight, residual, scale, scale_value, activation, eps, false));
 }
 
 }  // namespace
@@ -513,11 +524,12 @@ TORCH_LIBRARY_FRAGMENT(tgdn_b200, m) {
         "bool save=False) -> (Tensor, Tensor, Tensor)");
   m.def("gated_scan_bwd(Tensor x, Tensor g, Tensor dh, Tensor carry, Tensor? initial_state=None, Tensor? doc_map=None, SymInt documents=0, "
         "Tensor? dfinal=None) -> (Tensor, Tensor, Tensor)");
-  m.def("residual_norm_fwd(Tensor x, Tensor residual, Tensor? weight, Tensor? scale, float scale_value, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("residual_norm_fwd(Tensor x, Tensor residual, Tensor? weight, Tensor? scale, float scale_value, float eps, "
+        "bool save=False) -> (Tensor, Tensor, Tensor)");
   m.def("residual_norm_bwd(Tensor stream, Tensor? x, ScalarType x_type, Tensor? dy, Tensor? dstream, Tensor? weight, Tensor? scale, "
         "float scale_value, Tensor rstd, bool want_weight, bool want_scale) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("gated_norm_fwd(Tensor x, Tensor? gate, Tensor? weight, Tensor? residual, Tensor? scale, float scale_value, int activation, float eps) -> "
-        "(Tensor, Tensor)");
+  m.def("gated_norm_fwd(Tensor x, Tensor? gate, Tensor? weight, Tensor? residual, Tensor? scale, float scale_value, int activation, float eps, "
+        "bool save=False) -> (Tensor, Tensor)");
   m.def("gated_norm_bwd(Tensor x, Tensor? gate, Tensor dout, Tensor? weight, Tensor? scale, float scale_value, int activation, Tensor rstd, "
         "bool want_weight, bool want_scale) -> (Tensor, Tensor, Tensor, Tensor)");
 }

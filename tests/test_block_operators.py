@@ -28,12 +28,12 @@ def test_fake_kernels_give_the_real_shapes():
         assert doc_map.shape == (300,) and valid.shape == (1,)
         assert ops.gated_scan_fwd(x[:1], g[:1], None, doc_map, 4, True)[1].shape == (4, 40)
         r, w = like(2, 300, 40, dtype=F32), like(40)
-        y, stream, rstd = ops.residual_norm_fwd(x, r, w, w, 1.0, 1e-6)
+        y, stream, rstd = ops.residual_norm_fwd(x, r, w, w, 1.0, 1e-6, True)
         assert y.dtype == BF16 and stream.dtype == F32 and y.shape == stream.shape == x.shape and rstd.shape == (600,)
         dr, dxr, dw, dc = ops.residual_norm_bwd(stream, x, BF16, y, stream, w, w, 1.0, rstd, True, True)
         assert dr.dtype == F32 and dxr.dtype == BF16 and dw.shape == dc.shape == (40,)
         assert [t.numel() for t in ops.residual_norm_bwd(y, None, BF16, y, None, None, None, 1.0, rstd, False, False)[1:]] == [0, 0, 0]
-        out, rstd = ops.gated_norm_fwd(x, x, w, r, w, 1.0, 1, 1e-6)
+        out, rstd = ops.gated_norm_fwd(x, x, w, r, w, 1.0, 1, 1e-6, True)
         assert out.dtype == F32 and rstd.shape == (600,)
         dx, dz, dw, dc = ops.gated_norm_bwd(x, x, out, w, w, 1.0, 1, rstd, True, False)
         assert dx.shape == dz.shape == x.shape and dw.shape == (40,) and dc.numel() == 0
