@@ -209,7 +209,7 @@ int tgdn_bwd_matrix(const void* q, const void* k, const void* dO, const void* dU
 
 /* Rows of consecutive channels.  Row r starts (r / inner) * stride_outer + (r % inner) * stride_inner elements behind `data`; the scan
  * calls take a (B, T, D) tensor, stride_outer from batch row to batch row and stride_inner from token to token (inner is not read).
- * Strides may be zero; any alignment of whole elements will do (rows on 16-byte boundaries, or of pairs in the scan, are faster).
+ * Strides may be zero; any alignment of whole elements will do (in the scan, rows on 16-byte boundaries are faster).
  * data = NULL: no tensor. */
 typedef struct {
   const void* data;

@@ -219,3 +219,64 @@ def test_one_node_per_call_under_torch_compile():
         results.append([out.detach(), *torch.autograd.grad(out, leaves, torch.ones_like(out))])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_c_abi_entries_give_the_packages_bits():
+    """The entries as include/tgdn.h declares them, on the caller's buffers, against the operators that reach them through the package."""
+    L, p, ops = _lib.lib, _lib.ptr, torch.ops.tgdn_b200
+    gen = torch.Generator().manual_seed(4)
+    randn = lambda *s, dtype=F32: torch.randn(*s, generator=gen).to(dtype).cuda()
+    nan = lambda *s, dtype=F32: torch.full(s, float("nan"), dtype=dtype, device="cuda")
+    ids = {F32: 0, BF16: 1, torch.float16: 2}
+    rows = lambda t: ctypes.byref(_lib.Rows(t.data_ptr(), t.shape[-2] if t.dim() > 2 else t.shape[0], t.stride(0), t.stride(-2), ids[t.dtype]))
+    vec = lambda t: ctypes.byref(_lib.Vector(t.data_ptr(), ids[t.dtype]))
+
+    def call(name, *args):
+        _lib.check(getattr(L, name)(*[p(a) if torch.is_tensor(a) else a for a in args], _lib.stream_of(randn(1))), name)
+
+    for T, D, cu in ((200, 24, [0, 50, 51, 200]), (3000, 40, [0, 1000, 3000]), (3000, 33, None)):
+        x, g, dh, docs = randn(1, T, D, dtype=BF16), -randn(1, T, D).abs(), randn(1, T, D, dtype=BF16), len(cu) - 1 if cu else 0
+        initial, dfinal = randn(docs or 1, D), randn(docs or 1, D)
+        doc_map = None
+        if cu:
+            doc_map, valid = torch.full((T,), -1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.bool, device="cuda")
+            call("tgdn_scan_map", torch.tensor(cu, device="cuda"), 1, docs, T, doc_map, valid)
+            assert bool(valid) and doc_map.nonzero().flatten().tolist() == cu[:-1] and doc_map[cu[:-1]].tolist() == list(range(1, docs + 1))
+        floats = L.tgdn_scan_scratch_floats(1, T, D)
+        scratch = nan(floats) if floats else None
+        h, final, carry = nan(1, T, D, dtype=BF16), nan(docs or 1, D), nan(L.tgdn_scan_carry_floats(1, T, D))
+        call("tgdn_scan_fwd", rows(x), rows(g), doc_map, docs, 1, T, D, initial, h, final, carry, scratch, floats)
+        dx, dg, dinitial = nan(1, T, D, dtype=BF16), nan(1, T, D), nan(docs or 1, D)
+        call("tgdn_scan_bwd", rows(x), rows(g), rows(dh), doc_map, docs, 1, T, D, initial, carry, dfinal, dx, dg, dinitial, scratch, floats)
+        want = (*ops.gated_scan_fwd(x, g, initial, doc_map, docs, True, True), *ops.gated_scan_bwd(x, g, dh, carry, initial, doc_map, docs, dfinal))
+        assert all(torch.equal(a, b) for a, b in zip((h, final, carry, dx, dg, dinitial), want))
+        # without what is optional
+        h2 = nan(1, T, D, dtype=BF16)
+        call("tgdn_scan_fwd", rows(x), rows(g), doc_map, docs, 1, T, D, initial, h2, None, None, scratch, floats)
+        assert torch.equal(h, h2)
+    state, token = randn(3, 40), nan(3, 1, 40, dtype=BF16)
+    x, g, kept = randn(3, 1, 40, dtype=BF16), -randn(3, 1, 40).abs(), state.clone()
+    call("tgdn_scan_step", rows(x), rows(g), 3, 40, state, token)
+    assert torch.equal(gated_scan_decode(x, g, kept), token) and torch.equal(kept, state)
+
+    for R, N in ((70, 96), (9, 2001)):
+        x, r, z, dy, w, c = randn(R, N, dtype=BF16), randn(R, N), randn(R, N, dtype=BF16), randn(R, N, dtype=BF16), randn(N), randn(N, dtype=BF16)
+        y, stream, rstd = nan(R, N, dtype=BF16), nan(R, N), nan(R)
+        call("tgdn_residual_norm_fwd", rows(x), rows(r), vec(w), vec(c), 1.0, R, N, 1e-6, y, stream, rstd)
+        assert all(torch.equal(a, b) for a, b in zip((y, stream, rstd), ops.residual_norm_fwd(x, r, w, c, 1.0, 1e-6, True)))
+        floats = L.tgdn_norm_scratch_floats(R, N)
+        scratch, dr, dx, dw, dc = nan(floats), nan(R, N), nan(R, N, dtype=BF16), nan(N), nan(N, dtype=BF16)
+        call("tgdn_residual_norm_bwd", stream, 0, rows(x), 1, rows(dy), rows(r), vec(w), vec(c), 1.0, rstd, R, N, dr, dx, vec(dw), vec(dc), scratch, floats)
+        want = ops.residual_norm_bwd(stream, x, BF16, dy, r, w, c, 1.0, rstd, True, True)
+        assert all(torch.equal(a, b) for a, b in zip((dr, dx, dw, dc), want))
+        out, rstd = nan(R, N), nan(R)
+        call("tgdn_gated_norm_fwd", rows(x), rows(z), 1, vec(w), rows(r), vec(c), 1.0, R, N, 1e-6, out, 0, rstd)
+        assert all(torch.equal(a, b) for a, b in zip((out, rstd), ops.gated_norm_fwd(x, z, w, r, c, 1.0, 1, 1e-6, True)))
+        dx, dz, dw, dc = nan(R, N, dtype=BF16), nan(R, N, dtype=BF16), nan(N), nan(N, dtype=BF16)
+        call("tgdn_gated_norm_bwd", rows(x), rows(z), 1, rows(r), vec(w), vec(c), 1.0, rstd, R, N, dx, dz, vec(dw), vec(dc), scratch, floats)
+        want = ops.gated_norm_bwd(x, z, r, w, c, 1.0, 1, rstd, True, True)
+        assert all(torch.equal(a, b) for a, b in zip((dx, dz, dw, dc), want))
+        assert L.tgdn_residual_norm_bwd(p(stream), 0, rows(x), 1, rows(dy), None, vec(w), vec(c), 1.0, p(rstd), R, N, p(dr), p(dx), vec(dw), vec(dc),
+                                        p(scratch), 1, None) == -5
+    assert _lib.device_status() == 0
