@@ -362,7 +362,7 @@ __device__ __forceinline__ void bring_states(const ScanParams& p, const RowDocs&
     if (docs.starts_at(r)) x[r] = fma(a[r], load_f32<VEC>(p.initial + static_cast<int64_t>(docs.opened(r)) * p.D + c0, active), x[r]);
 }
 
-// The maps of the warps before one (or behind it, from the last warp back), composed in order.
+// The maps of the warps from one to before another (BACK: from one back to behind another), composed in order.
 template <int VEC, bool PACKED, bool BACK>
 __device__ __forceinline__ void compose(Map<VEC, PACKED>& m, const SharedMaps<VEC, PACKED>& maps, int buf, int lane, int from, int to) {
   if (BACK) {
@@ -373,6 +373,21 @@ __device__ __forceinline__ void compose(Map<VEC, PACKED>& m, const SharedMaps<VE
     for (int w = from; w < to; ++w) m.then(maps.get(buf, w, lane));
   }
 }
+// The same with the maps of all warps in registers first, which does not wait for shared memory at every step: where registers allow it (the
+// forward: single channels 10 % faster, pairs 3 %; the backward would spill, 68 -> 90 us at 64 channels x 4096).
+template <int VEC, bool PACKED>
+struct AllMaps {
+  Map<VEC, PACKED> m[SCAN_WARPS];
+  __device__ AllMaps(const SharedMaps<VEC, PACKED>& maps, int buf, int lane) {
+#pragma unroll
+    for (int w = 0; w < SCAN_WARPS; ++w) m[w] = maps.get(buf, w, lane);
+  }
+  __device__ void compose(Map<VEC, PACKED>& to, int lo, int hi) const {
+#pragma unroll
+    for (int w = 0; w < SCAN_WARPS; ++w)
+      if (w >= lo && w < hi) to.then(m[w]);
+  }
+};
 template <int VEC, bool PACKED>
 __device__ __forceinline__ void leave_map(const ScanParams& p, const Place<VEC>& at, int tile, const Map<VEC, PACKED>& m) {
   if (at.active) {

@@ -70,19 +70,20 @@ scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
     if (WAY == SCAN_MAPS) {
       if (warp == tile % SCAN_WARPS) {
         MapT whole = MapT::identity();
-        compose<VEC, PACKED, false>(whole, maps, buf, lane, 0, SCAN_WARPS);
+        AllMaps<VEC, PACKED>(maps, buf, lane).compose(whole, 0, SCAN_WARPS);
         leave_map<VEC, PACKED>(p, at, tile, whole);
       }
       continue;
     }
     // the maps of the warps before this one, and of all of the block; then the state before the warp's rows
     MapT whole = MapT::identity();
-    compose<VEC, PACKED, false>(whole, maps, buf, lane, 0, warp);
+    const AllMaps<VEC, PACKED> tile_maps(maps, buf, lane);
+    tile_maps.compose(whole, 0, warp);
     Lanes<VEC> mine = carry;
     whole.apply(mine);
     if (WAY == SCAN_WHOLE) {
       if (p.carry && warp == 0 && active) store_f32<VEC>(p.carry + at.at_tile(p, tile), carry);
-      compose<VEC, PACKED, false>(whole, maps, buf, lane, warp, SCAN_WARPS);
+      tile_maps.compose(whole, warp, SCAN_WARPS);
       whole.apply(carry);
     } else {
       carry = next_carry;
