@@ -15,7 +15,8 @@ __device__ __forceinline__ float reciprocal(float v) {
 }
 // The gate's activation and, where asked for, its slope, two channels at a time.  sigmoid(z) = 1 / (1 + 2^(-z log2 e)): the power of two
 // overflows to infinity below z = -88.7 and its reciprocal is zero there, as it should be; a quarter of the sum keeps the reciprocal in the
-// range that the hardware does not flush to zero.  Both hardware functions err by two units at most (a division in full precision costs eight instructions an element: 608 instead of 327 us at 65536 x 32 heads of 128).
+// range that the hardware does not flush to zero.  Both hardware functions err by two units at most; a
+// division in full precision is eight instructions an element more in kernels that are bound by their issue.
 template <bool SLOPE>
 __device__ __forceinline__ float2 gate_act(bool silu, float2 z, float2& slope) {
   const float2 t = __fmul2_rn(z, make_float2(-1.4426950408889634f, -1.4426950408889634f));

@@ -33,8 +33,8 @@ enum NormSize { NORM_GROUPS, NORM_WIDE, NORM_WIDEST };
 // Channels of a row a thread.  Sixteen, but for short rows of 32 bits, which would not fit the registers beside the next row's.
 constexpr int norm_channels(int bytes, int size) { return bytes == 4 && size == NORM_GROUPS ? 8 : 16; }
 // Threads of a block, and blocks an SM, that a kernel's registers are sized for: as many bytes on their way as possible without spilling.
-// Forward, rows of up to 512 threads: 80 registers do where both types have 16 bits (65536 x 2048, gated: 193 us with 100 registers, 150
-// with 80), not with a stream in 32 bits (32768 x 4096: 250 and 293 us).
+// Forward, rows of up to 512 threads: 80 registers do where both types have 16 bits (65536 x 2048, gated: 189 us with 100 registers, 150 with
+// 80 and the next round's gates on their way into L2), not with a stream in 32 bits (32768 x 4096: 264 us with 100 registers, 293 with 80).
 constexpr int norm_threads(int size, bool backward, bool small) {
   return size == NORM_GROUPS ? NORM_BLOCK : size == NORM_WIDEST ? 1024 : backward || !small ? 512 : 768;
 }
