@@ -237,8 +237,29 @@ struct alignas(16) SharedMaps {
     H[buf][part][lane] = m.H;
     if (PACKED && lane == 0) cut[buf][part] = m.cut;
   }
-  __device__ Map<VEC, PACKED> get(int buf, int part, int lane) const { return {A[buf][part][lane], H[buf][part][lane], PACKED ? cut[buf][part] : 0}; }
+  // CUTS: a document's border lies in the tile.
+  template <bool CUTS>
+  __device__ Map<VEC, CUTS> get(int buf, int part, int lane) const { return {A[buf][part][lane], H[buf][part][lane], CUTS ? cut[buf][part] : 0}; }
 };
+// The block's barrier between the maps' being written and read; true where a run of the tile holds a document's border.  The tiles that hold none do
+// without the selections and their registers (one packed row of 16384 x 8192 in bf16, forward: 313 -> 238 us; 8192 x 16384: 234 -> 176 us).
+template <bool PACKED>
+__device__ __forceinline__ bool maps_written(bool cut) {
+  if constexpr (PACKED) return __syncthreads_or(cut) != 0;
+  __syncthreads();
+  return false;
+}
+// f(true) for a tile with a document's border in it, else f(false), as constants.
+template <bool PACKED, typename F>
+__device__ __forceinline__ void by_cuts(bool cuts, F f) {
+  if constexpr (PACKED) {
+    if (cuts) {
+      f(std::true_type{});
+      return;
+    }
+  }
+  f(std::false_type{});
+}
 
 // The ring of tiles on their way: two to four stages of shared memory that the copy engine fills, each a block's rows of all its inputs, with
 // a barrier that completes when a stage's bytes are in.  One thread asks for a stage again as soon as all warps have what they need of it.
@@ -363,38 +384,39 @@ __device__ __forceinline__ void bring_states(const ScanParams& p, const RowDocs&
 }
 
 // The maps of the warps from one to before another (BACK: from one back to behind another), composed in order.
-template <int VEC, bool PACKED, bool BACK>
-__device__ __forceinline__ void compose(Map<VEC, PACKED>& m, const SharedMaps<VEC, PACKED>& maps, int buf, int lane, int from, int to) {
+template <bool BACK, bool CUTS, int VEC, bool PACKED>
+__device__ __forceinline__ void compose(Map<VEC, CUTS>& m, const SharedMaps<VEC, PACKED>& maps, int buf, int lane, int from, int to) {
   if (BACK) {
 #pragma unroll 2
-    for (int w = from; w > to; --w) m.then(maps.get(buf, w, lane));
+    for (int w = from; w > to; --w) m.then(maps.template get<CUTS>(buf, w, lane));
   } else {
 #pragma unroll 2
-    for (int w = from; w < to; ++w) m.then(maps.get(buf, w, lane));
+    for (int w = from; w < to; ++w) m.then(maps.template get<CUTS>(buf, w, lane));
   }
 }
 // The same with the maps of all warps in registers first, which does not wait for shared memory at every step: where registers allow it (the
-// forward: single channels 10 % faster, pairs 3 %; the backward would spill, 68 -> 90 us at 64 channels x 4096).
-template <int VEC, bool PACKED>
+// forward without a document's border: single channels 10 % faster, pairs 3 %; the backward would spill, 68 -> 90 us at 64 channels x 4096).
+template <int VEC, bool CUTS>
 struct AllMaps {
-  Map<VEC, PACKED> m[SCAN_WARPS];
+  Map<VEC, CUTS> m[SCAN_WARPS];
+  template <bool PACKED>
   __device__ AllMaps(const SharedMaps<VEC, PACKED>& maps, int buf, int lane) {
 #pragma unroll
-    for (int w = 0; w < SCAN_WARPS; ++w) m[w] = maps.get(buf, w, lane);
+    for (int w = 0; w < SCAN_WARPS; ++w) m[w] = maps.template get<CUTS>(buf, w, lane);
   }
-  __device__ void compose(Map<VEC, PACKED>& to, int lo, int hi) const {
+  __device__ void compose(Map<VEC, CUTS>& to, int lo, int hi) const {
 #pragma unroll
     for (int w = 0; w < SCAN_WARPS; ++w)
       if (w >= lo && w < hi) to.then(m[w]);
   }
 };
-template <int VEC, bool PACKED>
-__device__ __forceinline__ void leave_map(const ScanParams& p, const Place<VEC>& at, int tile, const Map<VEC, PACKED>& m) {
+template <int VEC, bool CUTS>
+__device__ __forceinline__ void leave_map(const ScanParams& p, const Place<VEC>& at, int tile, const Map<VEC, CUTS>& m) {
   if (at.active) {
     store_f32<VEC>(p.map_a + at.at_tile(p, tile), m.A);
     store_f32<VEC>(p.map_h + at.at_tile(p, tile), m.H);
   }
-  if (PACKED && at.slice0 == 0 && at.lane == 0) p.map_cut[tile] = m.cut;
+  if (p.map_cut && at.slice0 == 0 && at.lane == 0) p.map_cut[tile] = CUTS ? m.cut : 0;
 }
 
 }  // namespace tgdn
@@ -414,8 +436,9 @@ int scan_map_of(CUtensorMap* map, const ScanIn& in, int B, int T_, int D) {
                                   B > 1 ? in.sb : row * T_, 64, SCAN_TILE);
 }
 
-// `fixed`: static shared memory.  Two blocks an SM where there are more blocks than SMs and two stages leave room.
-template <bool RING, typename TX, typename TG, bool HAS_X, bool HAS_DH, typename Kernel>
+// `fixed`: static shared memory.  Two blocks an SM where the kernel has the registers for it (PER_SM), there are more blocks than SMs and two stages
+// leave room.
+template <bool RING, typename TX, typename TG, bool HAS_X, bool HAS_DH, int PER_SM, typename Kernel>
 int scan_launch(Kernel kernel, bool* configured, int fixed, ScanParams p, cudaStream_t s) {
   ScanMaps maps{};
   int bytes = 0;
@@ -429,7 +452,7 @@ int scan_launch(Kernel kernel, bool* configured, int fixed, ScanParams p, cudaSt
       if (const int rc = scan_map_of<TX>(&maps.dh, p.dh, p.B, p.T, p.D)) return rc;
     constexpr int stage = Ring<TX, TG, HAS_X, HAS_DH>::BYTES;
     const int two = (228 * 1024 / 2 - 1024 - fixed) / stage, one = (227 * 1024 - fixed) / stage;
-    p.stages = blocks > tgdn_sm_count() && two >= 2 ? two : one;
+    p.stages = PER_SM == 2 && blocks > tgdn_sm_count() && two >= 2 ? two : one;
     if (p.stages > SCAN_MAX_STAGES) p.stages = SCAN_MAX_STAGES;
     bytes = p.stages * stage;
     if (const int rc = tgdn_dynamic_smem(reinterpret_cast<const void*>(kernel), 227 * 1024 - fixed, configured)) return rc;

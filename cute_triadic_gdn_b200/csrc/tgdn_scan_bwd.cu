@@ -3,8 +3,13 @@
 
 namespace tgdn {
 
+// Blocks an SM that the registers are shared among.  Packed rows get one: at two, 128 registers a thread, they would spill 300 bytes and more, and
+// took longer even where there are two blocks for each SM (bf16, one row of 8192 x 16384: 467 -> 445 us; of 16384 x 8192, 128 blocks: 775 -> 396 us).
+// So do rows of more than four bytes a channel in x and g, whose stages leave no room for a second block; the maps alone fit twice.
+constexpr int bwd_per_sm(int bytes, bool packed, int way) { return way == SCAN_MAPS || (bytes == 4 && !packed) ? 2 : 1; }
+
 template <typename TX, typename TG, bool RING, bool PACKED, int WAY>
-__global__ void __launch_bounds__(32 * SCAN_WARPS, sizeof(TX) + sizeof(TG) == 4 ? 2 : 1)
+__global__ void __launch_bounds__(32 * SCAN_WARPS, bwd_per_sm(sizeof(TX) + sizeof(TG), PACKED, WAY))
 scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   constexpr int VEC = RING ? 2 : 1;
   constexpr bool STATES = WAY != SCAN_MAPS;      // (the reverse maps need neither x nor h)
@@ -87,20 +92,25 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
     back.A = run.A;
     maps[0].put(buf, warp, lane, back);
     if constexpr (STATES) maps[1].put(buf, warp, lane, run);
-    __syncthreads();
+    const bool tile_cuts = maps_written<PACKED>((run.cut | back.cut) != 0);
     if (asks && tile - p.stages >= at.lo && !ring.given_up()) ring.request((tile - p.stages) * SCAN_TILE);
 
     if constexpr (WAY == SCAN_MAPS) {
-      if (warp == tile % SCAN_WARPS) {
-        MapT whole = MapT::identity();
-        compose<VEC, PACKED, true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, -1);
-        leave_map<VEC, PACKED>(p, at, tile, whole);
-      }
+      if (warp == tile % SCAN_WARPS)
+        by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
+          constexpr bool CUTS = decltype(in_tile)::value;
+          Map<VEC, CUTS> whole = Map<VEC, CUTS>::identity();
+          compose<true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, -1);
+          leave_map(p, at, tile, whole);
+        });
       continue;
     } else {
-      MapT before = MapT::identity();
-      compose<VEC, PACKED, false>(before, maps[1], buf, lane, 0, warp);
-      before.apply(h);
+      by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
+        constexpr bool CUTS = decltype(in_tile)::value;
+        Map<VEC, CUTS> before = Map<VEC, CUTS>::identity();
+        compose<false>(before, maps[1], buf, lane, 0, warp);
+        before.apply(h);
+      });
       if (cuts) {                                // x becomes the state before its row
 #pragma unroll
         for (int r = 0; r < SCAN_ROWS; ++r) {
@@ -118,16 +128,18 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
           x[r] = last;
         }
       }
-      MapT whole = MapT::identity();
-      compose<VEC, PACKED, true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, warp);
       Lanes<VEC> mu = carry;
-      whole.apply(mu);
-      if (WAY == SCAN_WHOLE) {
-        compose<VEC, PACKED, true>(whole, maps[0], buf, lane, warp, -1);
-        whole.apply(carry);
-      } else {
-        carry = next_carry;
-      }
+      by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
+        constexpr bool CUTS = decltype(in_tile)::value;
+        Map<VEC, CUTS> whole = Map<VEC, CUTS>::identity();
+        compose<true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, warp);
+        whole.apply(mu);
+        if (WAY == SCAN_WHOLE) {
+          compose<true>(whole, maps[0], buf, lane, warp, -1);
+          whole.apply(carry);
+        }
+      });
+      if (WAY == SCAN_FINISH) carry = next_carry;
 
       const int64_t row = (static_cast<int64_t>(at.b) * p.T + t0) * p.D + c0;
       TX* dx = static_cast<TX*>(p.dx) + row;
@@ -166,7 +178,7 @@ struct Backward {
     static bool configured[64] = {false};
     constexpr int VEC = RING ? 2 : 1, fixed = (WAY == SCAN_MAPS ? 1 : 2) * static_cast<int>(sizeof(SharedMaps<VEC, PACKED>)) + 256;
     p.slices = (p.D + 32 * VEC - 1) / (32 * VEC);
-    return scan_launch<RING, TX, TG, WAY != SCAN_MAPS, true>(scan_bwd_kernel<TX, TG, RING, PACKED, WAY>, configured, fixed, p, s);
+    return scan_launch<RING, TX, TG, WAY != SCAN_MAPS, true, bwd_per_sm(sizeof(TX) + sizeof(TG), PACKED, WAY)>(scan_bwd_kernel<TX, TG, RING, PACKED, WAY>, configured, fixed, p, s);
   }
 };
 }  // namespace

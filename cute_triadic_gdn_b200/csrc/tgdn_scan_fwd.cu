@@ -3,10 +3,13 @@
 
 namespace tgdn {
 
+// Blocks an SM that the registers are shared among: two of 128 a thread with 16-bit rows, none of which spills.
+constexpr int fwd_per_sm(int x_bytes) { return x_bytes == 2 ? 2 : 1; }
+
 // RING: pairs of channels, tiles by the copy engine (rows of whole 16-byte pieces).  Otherwise single channels by plain loads of any
 // alignment, the next tile in registers.
 template <typename TX, typename TG, bool RING, bool PACKED, int WAY>
-__global__ void __launch_bounds__(32 * SCAN_WARPS, sizeof(TX) == 2 ? 2 : 1)
+__global__ void __launch_bounds__(32 * SCAN_WARPS, fwd_per_sm(sizeof(TX)))
 scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   constexpr int VEC = RING ? 2 : 1;
   using MapT = Map<VEC, PACKED>;
@@ -64,30 +67,41 @@ scan_fwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
       run_forward<false, VEC>(docs, a, x, run.A, run.H);
     }
     maps.put(buf, warp, lane, run);
-    __syncthreads();
+    const bool tile_cuts = maps_written<PACKED>(run.cut != 0);
     if (asks && tile + p.stages < at.hi && !ring.given_up()) ring.request((tile + p.stages) * SCAN_TILE);   // every warp has its rows
 
     if (WAY == SCAN_MAPS) {
-      if (warp == tile % SCAN_WARPS) {
-        MapT whole = MapT::identity();
-        AllMaps<VEC, PACKED>(maps, buf, lane).compose(whole, 0, SCAN_WARPS);
-        leave_map<VEC, PACKED>(p, at, tile, whole);
-      }
+      if (warp == tile % SCAN_WARPS)
+        by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
+          constexpr bool CUTS = decltype(in_tile)::value;
+          Map<VEC, CUTS> whole = Map<VEC, CUTS>::identity();
+          AllMaps<VEC, CUTS>(maps, buf, lane).compose(whole, 0, SCAN_WARPS);
+          leave_map(p, at, tile, whole);
+        });
       continue;
     }
-    // the maps of the warps before this one, and of all of the block; then the state before the warp's rows
-    MapT whole = MapT::identity();
-    const AllMaps<VEC, PACKED> tile_maps(maps, buf, lane);
-    tile_maps.compose(whole, 0, warp);
     Lanes<VEC> mine = carry;
-    whole.apply(mine);
-    if (WAY == SCAN_WHOLE) {
-      if (p.carry && warp == 0 && active) store_f32<VEC>(p.carry + at.at_tile(p, tile), carry);
-      tile_maps.compose(whole, warp, SCAN_WARPS);
-      whole.apply(carry);
-    } else {
-      carry = next_carry;
-    }
+    by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
+      // the maps of the warps before this one, and of all of the block; then the state before the warp's rows
+      constexpr bool CUTS = decltype(in_tile)::value;
+      Map<VEC, CUTS> whole = Map<VEC, CUTS>::identity();
+      const auto go = [&](auto composed) {
+        composed(whole, 0, warp);
+        whole.apply(mine);
+        if (WAY == SCAN_WHOLE) {
+          if (p.carry && warp == 0 && active) store_f32<VEC>(p.carry + at.at_tile(p, tile), carry);
+          composed(whole, warp, SCAN_WARPS);
+          whole.apply(carry);
+        }
+      };
+      if constexpr (CUTS) {
+        go([&](auto& to, int lo, int hi) { compose<false>(to, maps, buf, lane, lo, hi); });
+      } else {
+        const AllMaps<VEC, CUTS> tile_maps(maps, buf, lane);
+        go([&](auto& to, int lo, int hi) { tile_maps.compose(to, lo, hi); });
+      }
+    });
+    if (WAY == SCAN_FINISH) carry = next_carry;
 
     TX* out = static_cast<TX*>(p.h) + (static_cast<int64_t>(at.b) * p.T + t0) * p.D + c0;
     const int rows = active ? p.T - t0 : 0, stride = opaque(p.D);
@@ -126,7 +140,7 @@ struct Forward {
     static bool configured[64] = {false};
     constexpr int VEC = RING ? 2 : 1, fixed = static_cast<int>(sizeof(SharedMaps<VEC, PACKED>)) + 256;
     p.slices = (p.D + 32 * VEC - 1) / (32 * VEC);
-    return scan_launch<RING, TX, TG, true, false>(scan_fwd_kernel<TX, TG, RING, PACKED, WAY>, configured, fixed, p, s);
+    return scan_launch<RING, TX, TG, true, false, fwd_per_sm(sizeof(TX))>(scan_fwd_kernel<TX, TG, RING, PACKED, WAY>, configured, fixed, p, s);
   }
 };
 }  // namespace
