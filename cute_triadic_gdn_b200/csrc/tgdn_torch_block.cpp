@@ -224,6 +224,7 @@ Tensor scan_decode(const Tensor& x, const Tensor& g, const Tensor& state) {
   const SequenceRows xr(squeeze ? x : x.unsqueeze(1)), gr(squeeze ? g : g.unsqueeze(1));
   Tensor h = fresh(x.sizes(), x, x.scalar_type());
   check_rc(tgdn_scan_step(&xr.rows, &gr.rows, static_cast<int>(B), static_cast<int>(D), ptr<float>(state), ptr(h), stream_of(x)), "tgdn_scan_step");
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();      // a backward that still needs the state of before says so
   return h;
 }
 

@@ -259,6 +259,24 @@ def test_captured_in_a_graph_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(again, step(*leaves))) and not torch.equal(again[0], ref[0])
 
 
+def test_decode_counts_as_a_change_of_its_state():
+    x, g, initial, _, _ = make(2, 32, 8)
+    x.requires_grad_(True)
+    h = gated_scan_call(x, g, initial_state=initial)
+    before = initial._version
+    with torch.no_grad():
+        gated_scan_decode(x[:, :1].detach(), g[:, :1], initial)
+    assert initial._version == before + 1
+    with pytest.raises(RuntimeError, match="inplace"):                          # the backward of h would read the state of later
+        h.sum().backward()
+    with torch.inference_mode():
+        state = gated_scan_call(x.detach(), g, output_final_state=True)[1]
+        first = gated_scan_decode(x[:, :1].detach(), g[:, :1], state)
+    with torch.no_grad():
+        second = gated_scan_decode(x[:, :1].detach(), g[:, :1], state)          # a state of inference mode carries no count
+    assert first.shape == second.shape and not torch.equal(first, second)
+
+
 def test_unused_outputs_and_partial_gradients():
     x, g, initial, dh, dfinal = make(2, 70, 32)
     leaves = [t.requires_grad_(True) for t in (x, g, initial)]
