@@ -3,13 +3,17 @@
 
 namespace tgdn {
 
-// Blocks an SM that the registers are shared among.  Packed rows get one: at two, 128 registers a thread, they would spill 300 bytes and more, and
-// took longer even where there are two blocks for each SM (bf16, one row of 8192 x 16384: 467 -> 445 us; of 16384 x 8192, 128 blocks: 775 -> 396 us).
-// So do rows of more than four bytes a channel in x and g, whose stages leave no room for a second block; the maps alone fit twice.
-constexpr int bwd_per_sm(int bytes, bool packed, int way) { return way == SCAN_MAPS || (bytes == 4 && !packed) ? 2 : 1; }
+// Blocks an SM that the registers are shared among.  Pairs of channels in packed rows get one: at two, 128 registers a thread, they would spill 300
+// bytes and more, and took longer even where there are two blocks for each SM (bf16, one row of 8192 x 16384: 467 -> 445 us; of 16384 x 8192, 128
+// blocks: 775 -> 396 us).  So do pairs of more than four bytes in x and g, whose stages leave no room for a second block; the maps alone fit twice.
+// Single channels of 16-bit rows fit twice with few spills or none (f32 gates, 8 x 4096 x 1001: 189 -> 140 us; packed 16384 x 8001: 936 -> 734);
+// f32 rows keep their prefetch at one (8 x 4096 x 1001: 178 -> 150 us).
+constexpr int bwd_per_sm(int x_bytes, int g_bytes, bool ring, bool packed, int way) {
+  return way == SCAN_MAPS || (x_bytes == 2 && (!ring || (g_bytes == 2 && !packed))) ? 2 : 1;
+}
 
 template <typename TX, typename TG, bool RING, bool PACKED, int WAY>
-__global__ void __launch_bounds__(32 * SCAN_WARPS, bwd_per_sm(sizeof(TX) + sizeof(TG), PACKED, WAY))
+__global__ void __launch_bounds__(32 * SCAN_WARPS, bwd_per_sm(sizeof(TX), sizeof(TG), RING, PACKED, WAY))
 scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   constexpr int VEC = RING ? 2 : 1;
   constexpr bool STATES = WAY != SCAN_MAPS;      // (the reverse maps need neither x nor h)
@@ -178,7 +182,7 @@ struct Backward {
     static bool configured[64] = {false};
     constexpr int VEC = RING ? 2 : 1, fixed = (WAY == SCAN_MAPS ? 1 : 2) * static_cast<int>(sizeof(SharedMaps<VEC, PACKED>)) + 256;
     p.slices = (p.D + 32 * VEC - 1) / (32 * VEC);
-    return scan_launch<RING, TX, TG, WAY != SCAN_MAPS, true, bwd_per_sm(sizeof(TX) + sizeof(TG), PACKED, WAY)>(scan_bwd_kernel<TX, TG, RING, PACKED, WAY>, configured, fixed, p, s);
+    return scan_launch<RING, TX, TG, WAY != SCAN_MAPS, true, bwd_per_sm(sizeof(TX), sizeof(TG), RING, PACKED, WAY)>(scan_bwd_kernel<TX, TG, RING, PACKED, WAY>, configured, fixed, p, s);
   }
 };
 }  // namespace
