@@ -149,21 +149,24 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
       TX* dx = static_cast<TX*>(p.dx) + row;
       TG* dg = static_cast<TG*>(p.dg) + row;
       const int rows = active ? p.T - t0 : 0, stride = opaque(p.D);
-      Lanes<VEC> lam = cuts && docs.ends_at(SCAN_ROWS - 1) ? dh[SCAN_ROWS - 1] : add(dh[SCAN_ROWS - 1], mu);
+      by_cuts<PACKED>(cuts, [&](auto in_rows) {
+        constexpr bool CUTS = decltype(in_rows)::value;
+        Lanes<VEC> lam = CUTS && docs.ends_at(SCAN_ROWS - 1) ? dh[SCAN_ROWS - 1] : add(dh[SCAN_ROWS - 1], mu);
 #pragma unroll
-      for (int r = SCAN_ROWS - 1; r >= 0; --r) {
-        if (r < SCAN_ROWS - 1) lam = cuts && docs.ends_at(r) ? dh[r] : fma(a[r + 1], lam, dh[r]);
-        mu = mul(a[r], lam);
-        const Lanes<VEC> d = mul(mu, x[r]);
-        if (r < rows) {
-          store_f32_as<TX, VEC>(row_of(dx, r, stride), lam.v);
-          store_f32_as<TG, VEC>(row_of(dg, r, stride), d.v);
+        for (int r = SCAN_ROWS - 1; r >= 0; --r) {
+          if (r < SCAN_ROWS - 1) lam = CUTS && docs.ends_at(r) ? dh[r] : fma(a[r + 1], lam, dh[r]);
+          mu = mul(a[r], lam);
+          const Lanes<VEC> d = mul(mu, x[r]);
+          if (r < rows) {
+            store_f32_as<TX, VEC>(row_of(dx, r, stride), lam.v);
+            store_f32_as<TG, VEC>(row_of(dg, r, stride), d.v);
+          }
+          if (CUTS && p.dinitial && docs.starts_at(r)) {
+            const int doc = docs.opened(r);
+            if (active) store_f32<VEC>(p.dinitial + static_cast<int64_t>(doc) * p.D + c0, mu);
+          }
         }
-        if (cuts && p.dinitial && docs.starts_at(r)) {
-          const int doc = docs.opened(r);
-          if (active) store_f32<VEC>(p.dinitial + static_cast<int64_t>(doc) * p.D + c0, mu);
-        }
-      }
+      });
     }
   }
   if (WAY == SCAN_WHOLE && !PACKED && p.dinitial && warp == 0 && active) store_f32<VEC>(p.dinitial + at.state, carry);
