@@ -54,14 +54,17 @@ scan_fold_kernel(const float* A, const float* H, const int* cut, const float* st
       const int n = min(FOLD_TILES, tiles - lot * FOLD_TILES);
       int i = 0;
       for (; i + 8 <= n; i += 8) {               // eight maps in registers at a time, so that the walk waits for its own sums only
-        float a[8], h[8];
+        float a[8], h[8], low = 0.f, high = 0.f;
         int cuts = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           a[k] = s.A[i + k][lane];
           h[k] = s.H[i + k][lane];
           if (cut) cuts |= (s.cut[i + k] != 0) << k;
+          low = fminf(low, a[k]);
+          high = fmaxf(high, a[k]);
         }
+        if (!(low >= 0.f && high <= FLT_MAX)) break;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           *out = state;
@@ -69,10 +72,10 @@ scan_fold_kernel(const float* A, const float* H, const int* cut, const float* st
           state = cuts >> k & 1 ? h[k] : fmaf(a[k], state, h[k]);
         }
       }
-      for (; i < n; ++i) {
+      for (; i < n; ++i) {                       // the rest, and lots with factors out of range (tgdn_scan.cuh)
         *out = state;
         out += step;
-        state = cut && s.cut[i] ? s.H[i][lane] : fmaf(s.A[i][lane], state, s.H[i][lane]);
+        state = cut && s.cut[i] ? s.H[i][lane] : factor_apply(s.A[i][lane], state, s.H[i][lane]);
       }
     }
   }

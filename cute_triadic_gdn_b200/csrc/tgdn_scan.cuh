@@ -16,9 +16,10 @@
 // put its rounding into dg, and would have to be read in the place of x.
 //
 // Sums, products and states are f32.  Maps are composed in an order given by the tiles alone, so a sequence's results depend neither on what
-// runs beside it nor on the way taken.
+// runs beside it nor on the way taken.  Gates above zero may take A out of f32's range where no state leaves it: see "factors out of range".
 #pragma once
 
+#include <float.h>
 #include <type_traits>
 
 #include "tgdn_common.cuh"
@@ -211,6 +212,49 @@ __device__ __forceinline__ void unpack_rows(const RawRows<T, VEC>& raw, Lanes<VE
   for (int r = 0; r < SCAN_ROWS; ++r) raw.v[r].get(out[r].v);
 }
 
+// Factors out of range.  With gates above zero the product A of a run's decays may pass 2^128 where the states stay small, or zero, or shrink
+// again within the run.  A factor is never negative, so that one from 2^128 up to 2^319 is written as -A 2^-192; beyond that the smallest
+// state but zero overflows, and A is +infinity.  The blocks compose plainly, note in shared memory where a run's factor passes 2^15 (eight of
+// up to 2^15 stay in range in whatever order they are composed) and then walk their tiles once more by the wide forms: the same arithmetic
+// on plain factors, in the same order, 64 bits on the others.  (A test within the walk, with a branch, cost blocks that are alone on their
+// SM a third: 1 x 4096 x 4096 in bf16, backward, 72 -> 98 us; the note costs 0 to 2 %.  Where all
+// blocks walk twice, 8 x 4096 x 2048 takes 181 / 308 us instead of 76 / 136.)  Limits that remain: exp(g) is f32, and what is below
+// 2^-126, a state or a product of decays, counts as zero.
+__device__ __forceinline__ bool plain_factor(float a) { return a >= 0.f && a <= FLT_MAX; }
+__device__ __forceinline__ double factor_value(float a) { return a < 0.f ? static_cast<double>(a) * -0x1p192 : static_cast<double>(a); }
+__device__ __forceinline__ float factor_of(double v) {
+  if (!(v > FLT_MAX)) return static_cast<float>(v);
+  const float scaled = static_cast<float>(v * 0x1p-192);
+  return scaled <= FLT_MAX ? -scaled : scaled;
+}
+__device__ __forceinline__ float factor_times(float a, float b) {
+  const float product = a * b;
+  if (plain_factor(a) && plain_factor(b) && product <= FLT_MAX) return product;
+  if (a == 0.f) return b == b ? 0.f : b;         // (no 0 x infinity: what has come to zero does not grow, and what overflows stays so)
+  if (isinf(a)) return b == b ? a : b;
+  return factor_of(factor_value(a) * factor_value(b));
+}
+__device__ __forceinline__ float factor_apply(float a, float c, float h) {
+  if (plain_factor(a) || a != a) return fmaf(a, c, h);
+  if (c == 0.f) return h;
+  return isinf(a) ? fmaf(a, c, h) : static_cast<float>(factor_value(a) * c + h);
+}
+// The product of a run's decays where the plain one left the range on its way: exponents by steps of 2^64 beside the number.
+template <int VEC>
+__device__ __forceinline__ float factor_of_run(const Lanes<VEC> (&a)[SCAN_ROWS], int i) {
+  float m = 1.f;
+  int e = 0;
+#pragma unroll
+  for (int r = 0; r < SCAN_ROWS; ++r) {
+    const bool steep = a[r].v[i] > 0x1p32f, high = m > 0x1p32f, low = m < 0x1p-32f && e > 0;
+    m = (high ? m * 0x1p-64f : low ? m * 0x1p64f : m) * (steep ? a[r].v[i] * 0x1p-64f : a[r].v[i]);
+    e += steep + high - low;
+  }
+  double v = m;
+  for (; e > 0 && v <= 0x1p400; --e) v *= 0x1p64;
+  return factor_of(v);
+}
+
 // A map of a run of rows in a lane's channels: c -> A c + H, or c -> H where a document's border lies in the run (`cut`, one value for all
 // channels: a state that is infinite or NaN must not pass, so a factor of zero would not do).
 template <int VEC, bool PACKED>
@@ -224,6 +268,30 @@ struct Map {
     if (PACKED) cut |= n.cut;
   }
   __device__ void apply(Lanes<VEC>& c) const { c = PACKED && cut ? H : fma(A, c, H); }
+  __device__ bool moderate() const {             // (false for NaN)
+    bool all = A.v[0] <= 0x1p15f;
+#pragma unroll
+    for (int i = 1; i < VEC; ++i) all = all && A.v[i] <= 0x1p15f;
+    return all;
+  }
+  // The same with factors of any size: the run's own product `of` its decays, this map, then n, and a state through the map.
+  __device__ void widen(const Lanes<VEC> (&of)[SCAN_ROWS]) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (!plain_factor(A.v[i])) A.v[i] = factor_of_run<VEC>(of, i);
+  }
+  __device__ void then_wide(const Map& n) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      H.v[i] = PACKED && n.cut ? n.H.v[i] : factor_apply(n.A.v[i], H.v[i], n.H.v[i]);
+      A.v[i] = factor_times(A.v[i], n.A.v[i]);
+    }
+    if (PACKED) cut |= n.cut;
+  }
+  __device__ void apply_wide(Lanes<VEC>& c) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c.v[i] = PACKED && cut ? H.v[i] : factor_apply(A.v[i], c.v[i], H.v[i]);
+  }
 };
 
 // Maps in shared memory, of the block's warps; double-buffered, so that those of a tile are written while slower readers are still at the
@@ -277,6 +345,7 @@ struct ScanMaps {
 struct RingControl {
   uint64_t full[SCAN_MAX_STAGES];
   int abort;
+  int wide;                                      // a run's factor was too large for the plain forms
 };
 template <typename TX, typename TG, bool HAS_X, bool HAS_DH>
 struct Ring {
@@ -294,7 +363,7 @@ struct Ring {
       : maps(m), data(smem), control(ctl), wait_ctl{&ctl->abort, status}, c(c_), b(b_), stages(stages_) {
     if (threadIdx.x == 0) {
       for (int i = 0; i < stages; ++i) mbar_init(&control->full[i], 1);
-      control->abort = 0;
+      control->abort = control->wide = 0;
       mbar_fence_init();
     }
     __syncthreads();
@@ -410,6 +479,21 @@ struct AllMaps {
       if (w >= lo && w < hi) to.then(m[w]);
   }
 };
+// The same on factors of any size: the map of the warps [from, to), and the state `at_warp` behind those before `warp` from the state c before all.
+template <bool BACK, int VEC, bool CUTS, bool PACKED>
+__device__ __forceinline__ Map<VEC, CUTS> compose_wide(const SharedMaps<VEC, PACKED>& maps, int buf, int lane, int from, int to, int warp, const Lanes<VEC>& c,
+                                                       Lanes<VEC>& at_warp) {
+  Map<VEC, CUTS> m = Map<VEC, CUTS>::identity();
+#pragma unroll 1
+  for (int w = from;; w += BACK ? -1 : 1) {
+    if (w == warp) {
+      at_warp = c;
+      m.apply_wide(at_warp);
+    }
+    if (w == to) return m;
+    m.then_wide(maps.template get<CUTS>(buf, w, lane));
+  }
+}
 template <int VEC, bool CUTS>
 __device__ __forceinline__ void leave_map(const ScanParams& p, const Place<VEC>& at, int tile, const Map<VEC, CUTS>& m) {
   if (at.active) {

@@ -12,26 +12,19 @@ constexpr int bwd_per_sm(int x_bytes, int g_bytes, bool ring, bool packed, int w
   return way == SCAN_MAPS || (x_bytes == 2 && (!ring || (g_bytes == 2 && !packed))) ? 2 : 1;
 }
 
-template <typename TX, typename TG, bool RING, bool PACKED, int WAY>
-__global__ void __launch_bounds__(32 * SCAN_WARPS, bwd_per_sm(sizeof(TX), sizeof(TG), RING, PACKED, WAY))
-scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
-  constexpr int VEC = RING ? 2 : 1;
+// WIDE: once more over the block's tiles, with factors out of range.
+template <typename TX, typename TG, bool RING, bool PACKED, int WAY, bool WIDE, int VEC>
+__device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, const Place<VEC>& at, SharedMaps<VEC, PACKED>* maps, Ring<TX, TG, WAY != SCAN_MAPS, true>& ring) {
   constexpr bool STATES = WAY != SCAN_MAPS;      // (the reverse maps need neither x nor h)
   using MapT = Map<VEC, PACKED>;
   using RingT = Ring<TX, TG, STATES, true>;
-  extern __shared__ __align__(128) uint8_t dynamic[];
-  __shared__ SharedMaps<VEC, PACKED> maps[STATES ? 2 : 1];     // reverse, forward
-  __shared__ RingControl control;
-  const Place<VEC> at(p, WAY == SCAN_FINISH);
   const int lane = at.lane, warp = at.warp, c0 = at.c0;
-  const bool active = at.active;
+  const bool active = at.active, asks = RING && threadIdx.x == 0;
   const int64_t xb = at.b * p.x.sb + (active ? c0 : 0), gb = at.b * p.g.sb + (active ? c0 : 0), hb = at.b * p.dh.sb + (active ? c0 : 0);
   // mu behind the tile, the same in every warp
   Lanes<VEC> carry = load_f32<VEC>(p.dfinal + at.state, WAY == SCAN_WHOLE && !PACKED && p.dfinal && active);
   if (WAY == SCAN_FINISH) carry = load_f32<VEC>(p.mu + at.at_tile(p, at.hi - 1), active);
 
-  RingT ring(tensors, dynamic, &control, p.status, at.slice0, at.b, RING ? p.stages : 0);
-  const bool asks = RING && threadIdx.x == 0;
   RawRows<TX, VEC> xr, hr;
   RawRows<TG, VEC> gr;
   auto request = [&](int t0) {
@@ -44,7 +37,7 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   auto saved = [&](int tile) { return load_f32<VEC>(p.carry + at.at_tile(p, tile), STATES && active && tile >= at.lo); };   // the state before a tile
   if (asks)
     for (int n = 0; n < p.stages && at.hi - 1 - n >= at.lo; ++n) ring.request((at.hi - 1 - n) * SCAN_TILE);
-  request((at.hi - 1) * SCAN_TILE + warp * SCAN_ROWS);
+  if (!WIDE) request((at.hi - 1) * SCAN_TILE + warp * SCAN_ROWS);   // (the second walk has no registers for rows ahead)
   int code = row_code<PACKED>(p, (at.hi - 1) * SCAN_TILE + warp * SCAN_ROWS, lane);
   Lanes<VEC> next_h = saved(at.hi - 1);
   for (int tile = at.hi - 1; tile >= at.lo; --tile) {
@@ -58,10 +51,11 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
       take_rows<TX, VEC>(here + RingT::DH_AT, warp, lane, hr);
       ring.advance();
     }
+    if (WIDE) request(t0);
     if constexpr (STATES) unpack_rows<TX, VEC>(xr, x);
     unpack_rows<TG, VEC>(gr, a);
     unpack_rows<TX, VEC>(hr, dh);
-    if (more) request(t0 - SCAN_TILE);
+    if (!WIDE && more) request(t0 - SCAN_TILE);
     const RowDocs docs = row_docs<PACKED>(p, t0, code);
     const bool cuts = PACKED && docs.any();
     Lanes<VEC> h = next_h;
@@ -93,6 +87,8 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
     if constexpr (!STATES)
 #pragma unroll
       for (int r = 0; r < SCAN_ROWS; ++r) run.A = mul(run.A, a[r]);
+    if (WIDE) run.widen(a);
+    else if (!run.moderate()) ring.control->wide = 1;
     back.A = run.A;
     maps[0].put(buf, warp, lane, back);
     if constexpr (STATES) maps[1].put(buf, warp, lane, run);
@@ -104,16 +100,25 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
         by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
           constexpr bool CUTS = decltype(in_tile)::value;
           Map<VEC, CUTS> whole = Map<VEC, CUTS>::identity();
-          compose<true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, -1);
+          if constexpr (WIDE) {
+            whole = compose_wide<true, VEC, CUTS>(maps[0], buf, lane, SCAN_WARPS - 1, -1, SCAN_WARPS, carry, carry);
+          } else {
+            compose<true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, -1);
+          }
           leave_map(p, at, tile, whole);
         });
       continue;
     } else {
       by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
         constexpr bool CUTS = decltype(in_tile)::value;
-        Map<VEC, CUTS> before = Map<VEC, CUTS>::identity();
-        compose<false>(before, maps[1], buf, lane, 0, warp);
-        before.apply(h);
+        if constexpr (WIDE) {
+          const Lanes<VEC> first = h;
+          compose_wide<false, VEC, CUTS>(maps[1], buf, lane, 0, warp, warp, first, h);
+        } else {
+          Map<VEC, CUTS> before = Map<VEC, CUTS>::identity();
+          compose<false>(before, maps[1], buf, lane, 0, warp);
+          before.apply(h);
+        }
       });
       if (cuts) {                                // x becomes the state before its row
 #pragma unroll
@@ -136,11 +141,16 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
       by_cuts<PACKED>(tile_cuts, [&](auto in_tile) {
         constexpr bool CUTS = decltype(in_tile)::value;
         Map<VEC, CUTS> whole = Map<VEC, CUTS>::identity();
-        compose<true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, warp);
-        whole.apply(mu);
-        if (WAY == SCAN_WHOLE) {
-          compose<true>(whole, maps[0], buf, lane, warp, -1);
-          whole.apply(carry);
+        if constexpr (WIDE) {
+          whole = compose_wide<true, VEC, CUTS>(maps[0], buf, lane, SCAN_WARPS - 1, WAY == SCAN_WHOLE ? -1 : warp, warp, carry, mu);
+          if (WAY == SCAN_WHOLE) whole.apply_wide(carry);
+        } else {
+          compose<true>(whole, maps[0], buf, lane, SCAN_WARPS - 1, warp);
+          whole.apply(mu);
+          if (WAY == SCAN_WHOLE) {
+            compose<true>(whole, maps[0], buf, lane, warp, -1);
+            whole.apply(carry);
+          }
         }
       });
       if (WAY == SCAN_FINISH) carry = next_carry;
@@ -171,6 +181,27 @@ scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, ScanParams p) {
   }
   if (WAY == SCAN_WHOLE && !PACKED && p.dinitial && warp == 0 && active) store_f32<VEC>(p.dinitial + at.state, carry);
   if (asks && ring.given_up()) ring.drain();
+}
+// A function of its own, so that the plain walk keeps its registers.
+template <typename TX, typename TG, bool RING, bool PACKED, int WAY, int VEC>
+__device__ __noinline__ void scan_bwd_again(const ScanParams& p, SharedMaps<VEC, PACKED>* maps, Ring<TX, TG, WAY != SCAN_MAPS, true> ring) {
+  const Place<VEC> at(p, WAY == SCAN_FINISH);
+  scan_bwd_walk<TX, TG, RING, PACKED, WAY, true, VEC>(p, at, maps, ring);
+}
+
+template <typename TX, typename TG, bool RING, bool PACKED, int WAY>
+__global__ void __launch_bounds__(32 * SCAN_WARPS, bwd_per_sm(sizeof(TX), sizeof(TG), RING, PACKED, WAY))
+scan_bwd_kernel(const __grid_constant__ ScanMaps tensors, const __grid_constant__ ScanParams p) {
+  constexpr int VEC = RING ? 2 : 1;
+  constexpr bool STATES = WAY != SCAN_MAPS;
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  __shared__ SharedMaps<VEC, PACKED> maps[STATES ? 2 : 1];     // reverse, forward
+  __shared__ RingControl control;
+  const Place<VEC> at(p, WAY == SCAN_FINISH);
+  Ring<TX, TG, STATES, true> ring(tensors, dynamic, &control, p.status, at.slice0, at.b, RING ? p.stages : 0);
+  scan_bwd_walk<TX, TG, RING, PACKED, WAY, false, VEC>(p, at, maps, ring);
+  __syncthreads();
+  if (control.wide && !ring.given_up()) scan_bwd_again<TX, TG, RING, PACKED, WAY, VEC>(p, maps, ring);   // (a block that gave up asks for nothing more)
 }
 
 }  // namespace tgdn

@@ -37,9 +37,10 @@ def _bwd_fake(x, g, dh, carry, initial_state=None, doc_map=None, documents=0, df
 def gated_scan_call(x, g, cu_seqlens=None, *, initial_state=None, output_final_state=False):
     """h (B, T, D) of h[t] = exp(g[t]) h[t-1] + x[t], every channel by itself, states in f32; h has x's type.
 
-    x: (B, T, D) f32, bf16 or f16; g: logs of decays (g <= 0 for a state that forgets; -inf drops a finite state), f32 or of x's type.  Any strides over
-    batch and tokens are read in place (a slice of a projection, an expanded gate).  `initial_state`: f32 (sequences, D), zero if not given;
-    with `output_final_state=True` the call returns (h, final_state).  Differentiable in x, g and initial_state, through h and final_state, so
+    x: (B, T, D) f32, bf16 or f16; g: logs of decays (g <= 0 for a state that forgets; above zero it grows; -inf drops a finite state), f32 or
+    of x's type.  exp(g) and the states are f32: a gate above 88.7 is infinite growth, and a state, or a product of decays, below 2^-126 counts
+    as zero.  Any strides over batch and tokens are read in place (a slice of a projection, an expanded gate).  `initial_state`: f32
+    (sequences, D), zero if not given; with `output_final_state=True` the call returns (h, final_state).  Differentiable in x, g and initial_state, through h and final_state, so
     that sequences can be processed in segments.
 
     With cu_seqlens the inputs are one packed row (1, T, D) as in `gdn_joint_call`: contiguous int32/int64 CUDA offsets that start at 0, end

@@ -222,7 +222,8 @@ typedef struct {
   int type;
 } tgdn_vector;
 
-/* Gated linear recurrence per channel: h[t] = exp(g[t]) h[t-1] + x[t] over (B, T, D), states f32.  (x, g): types f32 with f32, bf16 or
+/* Gated linear recurrence per channel: h[t] = exp(g[t]) h[t-1] + x[t] over (B, T, D), states and exp(g) f32; the product of the decays of
+ * several tokens may pass f32's range, and counts as zero below 2^-126.  (x, g): types f32 with f32, bf16 or
  * f16 with themselves or f32.  Dense rows: map = NULL, sequences = B.  Packed rows: B = 1, map (T) int32 from tgdn_scan_map, sequences =
  * n_docs; every document starts from its own state.  initial: f32 (sequences, D) or NULL (zero); final_state: f32 (sequences, D) or NULL;
  * carry: tgdn_scan_carry_floats(B, T, D) floats that the backward reads (the state before every TGDN_SCAN_TILE tokens), or NULL.
