@@ -6,7 +6,8 @@ namespace tgdn {
 
 // The states between the tiles from the tiles' maps: carry[i] = the state before tile i (REVERSE: behind it), end = the state behind the last
 // (before the first).  A block has 32 channels of a batch row; all warps bring the maps of 64 tiles at a time into shared memory, three
-// lots ahead, and the first walks over them: a fused multiply-add a tile, 1024 tiles of 1024 channels in 21 us (a fortieth of the forward and backward around it).
+// lots ahead, and the first walks over them: a fused multiply-add a tile, 1024 tiles of 1024 channels in 26 us with cold
+// caches (a thirtieth of the forward and backward around it; 24 without the look at the factors' range).
 constexpr int FOLD_TILES = 64, FOLD_STAGES = 4, FOLD_THREADS = 256;
 struct FoldStage {
   float A[FOLD_TILES][32], H[FOLD_TILES][32];
@@ -52,19 +53,20 @@ scan_fold_kernel(const float* A, const float* H, const int* cut, const float* st
     if (warp == 0 && active) {
       const FoldStage& s = stages[lot % FOLD_STAGES];
       const int n = min(FOLD_TILES, tiles - lot * FOLD_TILES);
+      const float first = state;
+      float* const from = out;
+      uint32_t largest = 0u;                     // of the factors' bits: plain ones are below infinity's
       int i = 0;
       for (; i + 8 <= n; i += 8) {               // eight maps in registers at a time, so that the walk waits for its own sums only
-        float a[8], h[8], low = 0.f, high = 0.f;
+        float a[8], h[8];
         int cuts = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           a[k] = s.A[i + k][lane];
           h[k] = s.H[i + k][lane];
           if (cut) cuts |= (s.cut[i + k] != 0) << k;
-          low = fminf(low, a[k]);
-          high = fmaxf(high, a[k]);
+          largest = max(largest, __float_as_uint(a[k]));
         }
-        if (!(low >= 0.f && high <= FLT_MAX)) break;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           *out = state;
@@ -72,10 +74,21 @@ scan_fold_kernel(const float* A, const float* H, const int* cut, const float* st
           state = cuts >> k & 1 ? h[k] : fmaf(a[k], state, h[k]);
         }
       }
-      for (; i < n; ++i) {                       // the rest, and lots with factors out of range (tgdn_scan.cuh)
+      for (; i < n; ++i) {
         *out = state;
         out += step;
-        state = cut && s.cut[i] ? s.H[i][lane] : factor_apply(s.A[i][lane], state, s.H[i][lane]);
+        largest = max(largest, __float_as_uint(s.A[i][lane]));
+        state = cut && s.cut[i] ? s.H[i][lane] : fmaf(s.A[i][lane], state, s.H[i][lane]);
+      }
+      if (largest >= 0x7f800000u) {              // once more for factors out of range (tgdn_scan.cuh); a test every eight maps took a third longer
+        state = first;
+        out = from;
+#pragma unroll 1
+        for (i = 0; i < n; ++i) {
+          *out = state;
+          out += step;
+          state = cut && s.cut[i] ? s.H[i][lane] : factor_apply(s.A[i][lane], state, s.H[i][lane]);
+        }
       }
     }
   }
