@@ -61,7 +61,7 @@ def residual_norm_call(x, residual, weight=None, scale=None, eps=1e-6):
 
     over the last axis (at most 16384 channels).  x: (..., N) f32, bf16 or f16, the output of the block before; residual: x's shape, f32 or
     x's type; `stream` has the residual's type (the next call's residual), `y` x's.  The norm is taken of the sum before it is rounded to the
-    stream's type; the backward forms it from the stream as stored.  weight: (N), ones if not given; scale: a number or a vector (N), one if not
+    stream's type; the backward forms it from the stream as stored (with a 16-bit stream, gradients of f32 vectors are as good as its type).  weight: (N), ones if not given; scale: a number or a vector (N), one if not
     given.  Differentiable in all four tensors.  Rows are read in place where their strides allow it."""
     vector, value = _scale(scale)
     if not torch.compiler.is_compiling():

@@ -14,7 +14,9 @@
 // small kernel: no atomics, the same bits every time.
 //
 // Sums, norms and products are f32; a rounding to the tensors' types happens once, at each store.  The norm before a block is taken of
-// the sum before its rounding to the stream's type.
+// the sum before its rounding to the stream's type.  Its backward forms n from the stream as stored, which saves reading x and the residual
+// again: with a stream in 16 bits every n is off by up to half a step of that type, which gradients in 16 bits do not show, and which
+// dweight and dscale in f32 carry as a mean over the rows.
 #pragma once
 
 #include <initializer_list>
@@ -32,7 +34,10 @@ constexpr int NORM_MAX_WARPS = 32;
 enum NormSize { NORM_GROUPS, NORM_WIDE, NORM_WIDEST };
 // Channels of a row a thread.  Sixteen, but for short rows of 32 bits, which would not fit the registers beside the next row's.
 constexpr int norm_channels(int bytes, int size) { return bytes == 4 && size == NORM_GROUPS ? 8 : 16; }
-// Threads of a block, and blocks an SM, that a kernel's registers are sized for: as many bytes on their way as possible without spilling.
+// Threads of a block, and blocks an SM, that a kernel's registers are sized for, by time: as many bytes on their way as possible.  Rows of up to
+// 8192 channels on vectors' borders spill nothing forward and up to 36 bytes a thread backward, but for the residual norm of heads (44 to 228);
+// rows of odd length up to 336 bytes.  Above 8192 channels 64 registers a thread are too few for sixteen channels (up to 400 bytes forward, 328
+// to 588 backward, rows of odd length up to 1420); most kernels of single channels spill too (up to 908).
 // Forward, rows of up to 512 threads: 80 registers do where both types have 16 bits (65536 x 2048, gated: 189 us with 100 registers, 150 with
 // 80 and the next round's gates on their way into L2), not with a stream in 32 bits (32768 x 4096: 264 us with 100 registers, 293 with 80).
 constexpr int norm_threads(int size, bool backward, bool small) {

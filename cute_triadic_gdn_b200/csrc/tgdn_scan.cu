@@ -153,6 +153,7 @@ namespace {
 // 0.019 us a tile and slice.  So the split way is ahead from 6 tiles on for one slice (64 channels x 16384: 163 -> 11 us forward), from 17 for
 // 64 slices (4096 channels x 4096: 44 -> 36 us, x 1024: 12 -> 13 us), and not above 90 (6144 x 4096: 45 and 59 us).  Four more launches of a
 // forward and backward cost the host 15 us where it is what a call waits for (3 x 1000 x 333: 69 and 84 us a step): twice the tiles.
+// Slices are counted as 64 channels for every kernel, as the measurements are; kernels of single channels have twice the blocks.
 bool scan_splits(int B, int T, int D) {
   const int64_t units = static_cast<int64_t>(B) * ((D + 63) / 64), tiles = (T - 1) / SCAN_TILE + 1, spare = tgdn_sm_count() * 5 / 8 - units;
   return spare > 0 && tiles * spare > 1000;

@@ -103,7 +103,7 @@ __device__ __forceinline__ float power_of_two(float t) {
 // exp(g).  Near zero as 1 + (g + g^2/2 + ...): the sum is rounded once, to nearest, while the hardware's power of two errs by up to two
 // units to one side, and such errors add up over as many tokens as the state remembers (a thousand tokens at g = -1e-3: 2e-5 where
 // roundings to nearest leave 1e-6).  Beyond 1/8 a state remembers eight tokens at most and the power of two is good enough.  The series
-// to the fifth power is 2^-28 off at 1/8.  (Decays below 2^-126 are zero.)
+// to the fifth power is 2^-27.3 off at -1/8, a tenth of a rounding's 2^-24, and 2^-33.4 at -1/16.  (Decays below 2^-126 are zero.)
 template <int VEC>
 __device__ __forceinline__ Lanes<VEC> decay(const Lanes<VEC>& g) {
   Lanes<VEC> s = fma(g, all<VEC>(1.f / 120.f), all<VEC>(1.f / 24.f));
